@@ -50,6 +50,7 @@ enum mi355x_type {
     MI355X_TYPE_Q8_0 = 8,
     MI355X_TYPE_Q4_K = 12,
     MI355X_TYPE_I32  = 26,
+    MI355X_TYPE_BF16 = 30,      /* the paged K/V cache and its attentions only: every other op answers MI355X_E_UNSUPPORTED */
 };
 
 /* mirrors the fields of struct ggml_tensor (ggml/include/ggml.h:673-705) a kernel needs */
@@ -318,6 +319,101 @@ MI355X_API int mi355x_flash_attn_ext_prep_rows(mi355x_ctx * ctx, const mi355x_te
 MI355X_API int mi355x_flash_attn_ext_exact(mi355x_ctx * ctx, const mi355x_tensor * q, const mi355x_tensor * k,
                                            const mi355x_tensor * v, const mi355x_tensor * mask /* nullable */,
                                            const mi355x_tensor * dst, float scale, int nth);
+
+/* ---- a K/V cache of pages shared by many streams, and the attentions that read it (csrc/kernels/kv_cache.hip, attn_paged.hip, attn_packed.hip) ----
+ * Two pools of pages (page_size keys of every K/V head; keys and values of one layer) and, in device memory, a row of page numbers for each
+ * sequence, the sequences' lengths and the number of rows that hold each page.  Key j of sequence s lies in page table[s][j / page_size], at
+ * j % page_size.  Pages without a holder are free; the calls below hand out the LOWEST free ones, in the order of their list, so that equal
+ * states and lists give equal tables.  All of it is the caller's memory and stays where it is: the calls only launch kernels on the context's
+ * stream (nothing is allocated, copied to the host or waited for), so they can be captured into a graph and replayed with new lists.
+ *
+ * What a call finds wrong with DEVICE values — a sequence >= n_seq, one named twice, offsets that fall or leave the rows, too few free pages, a
+ * full table row — it reports in *status (OR of enum mi355x_kv_status, never cleared by a call) and then changes nothing of the cache.  Lists may
+ * hold -1 for an entry to be left out (a padded batch).  Calls that change one cache follow one another (one stream, or ordered by events). */
+enum mi355x_kv_status {
+    MI355X_KV_BAD_ARG      = 1,    /* a list entry, offset, length or table entry out of range, or a sequence named twice */
+    MI355X_KV_ROW_FULL     = 2,    /* a sequence would need more than max_pages pages */
+    MI355X_KV_OUT_OF_PAGES = 4,    /* fewer free pages than the call needs */
+};
+typedef struct mi355x_kv_cache {
+    void *    k;                   /* pools: element (d, key, head, page) at page*nb_page + head*nb_head + key*nb_key + d*2 bytes, equally in both; 16-byte aligned */
+    void *    v;
+    int32_t   type;                /* F16 or BF16 */
+    int32_t   head_dim;            /* 64 or 128 */
+    int32_t   n_head_kv;           /* n_head_kv * head_dim <= 32768 */
+    int32_t   page_size;           /* keys per page: a power of two, 1 .. 4096 */
+    int32_t   n_pages;
+    int32_t   n_seq;               /* rows of the table, <= 262144 */
+    int32_t   max_pages;           /* entries of a row */
+    int32_t   reserved;
+    int64_t   nb_key, nb_head, nb_page;    /* byte strides, multiples of 16: heads before keys or keys before heads */
+    int32_t * table;               /* device [n_seq][max_pages], -1 behind a sequence's pages */
+    int32_t * len;                 /* device [n_seq]: keys held */
+    int32_t * ref;                 /* device [n_pages]: rows that hold the page, 0 = free */
+    int32_t * status;              /* device [1] */
+    void *    work;                /* device, mi355x_kv_work_bytes(n_seq, n_pages): contents mean nothing between calls */
+} mi355x_kv_cache;
+MI355X_API size_t mi355x_kv_work_bytes(int n_seq, int n_pages);
+/* every sequence empty, every page free, *status = 0 (the pools are not touched) */
+MI355X_API int mi355x_kv_reset(mi355x_ctx * ctx, const mi355x_kv_cache * c);
+/* rows cu[i] .. cu[i+1]-1 of k and v [head_dim, n_head_kv, n_rows] (F32 / F16 / BF16, rounded to the cache's type) go behind what sequence seq[i]
+ * holds; n <= n_seq.  seq [n] and cu [n+1] in device memory.  Pages are taken as needed; a partly filled last page that other rows hold too
+ * is copied to a page of its own first (by every sequence that appends to it).  All entries or, where *status says why, none. */
+MI355X_API int mi355x_kv_append(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n, const int32_t * seq, const int32_t * cu,
+                                const mi355x_tensor * k, const mi355x_tensor * v);
+/* sequence seq[i] keeps its first keep[i] keys (0: it is freed; more than it holds: nothing happens); pages behind them leave its row.  The same
+ * sequence twice: the smaller keep holds.  Entries that are not valid are left out and reported. */
+MI355X_API int mi355x_kv_truncate(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n, const int32_t * seq, const int32_t * keep);
+/* sequence dst[i] becomes what src[i] was BEFORE the call (beam search: the reference's sequence copies, src/whisper.cpp:1170-1190) without copying
+ * keys: both rows hold the same pages.  What dst[i] held leaves its row; src[i] = -1 leaves it empty.  A dst named twice is refused; n <= 8192. */
+MI355X_API int mi355x_kv_fork(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n, const int32_t * src, const int32_t * dst);
+/* every held page of `from`, in ascending order, becomes page 0, 1, 2 .. of `to` (another pool with its own table, len, ref and work; the same type,
+ * dims and n_seq, any strides, n_pages and max_pages >= from's): a fragmented cache made dense, or moved to a larger or a smaller pool.  Shared
+ * pages stay shared.  `from` keeps its contents.  Too few pages in `to`: its *status says so and it stays as it was. */
+MI355X_API int mi355x_kv_compact(mi355x_ctx * ctx, const mi355x_kv_cache * from, const mi355x_kv_cache * to);
+
+/* attention of ONE new token of each of n streams over the cache: query i, of sequence seq[i] (NULL: of sequence i), sees the keys that the sequence
+ * holds (its own among them: append first), the last `window` of them if window > 0.
+ *   dst[:, h, i] = softmax_j(scale * q[:, h, i] . k_j) v_j     head h reads K/V head h / (n_head / n_head_kv)
+ * An empty sequence and an entry of -1 give zeros.  q, dst: [head_dim, n_head, n], F32 / F16 / BF16, nb[0] = element, 16-byte aligned.  F32 queries
+ * count as such (split into 2 or 3 terms of the cache's type, |q| <= 65504 with F16 caches), sums and softmax are F32.  Rows past a sequence's end
+ * and before its window are never read.  max_len: what the caller knows of the lengths (0: nothing; the table's width); it decides how far the work
+ * is split over the keys, longer sequences are still complete.  work: mi355x_attn_paged_work_bytes(...) bytes of device memory (NULL if that is
+ * 0); calls that may run at the same time need their own.  A page number outside the pool is reported in *status (that row's result means nothing). */
+typedef struct mi355x_attn_paged_desc {
+    mi355x_tensor   q, dst;
+    const int32_t * seq;           /* device [n] or NULL */
+    float           scale;
+    int32_t         window;
+    int32_t         max_len;
+    int32_t         reserved;
+    void *          work;
+    size_t          work_bytes;
+} mi355x_attn_paged_desc;
+MI355X_API size_t mi355x_attn_paged_work_bytes(const mi355x_kv_cache * c, int n, int n_head, int max_len);
+MI355X_API int    mi355x_attn_paged(mi355x_ctx * ctx, const mi355x_kv_cache * c, const mi355x_attn_paged_desc * d);
+
+/* attention of the rows of n packed sequences: rows cu_q[i] .. cu_q[i+1]-1 of q are the LAST rows of sequence i, whose keys are rows cu_k[i] ..
+ * cu_k[i+1]-1 of k and v (cu_k NULL: cu_q), or, with a cache, the keys that sequence seq[i] of the cache holds (seq NULL: i; -1: none).  With Q rows and L
+ * keys, row r sees the keys j <= L - Q + r (causal; all otherwise), and of them those with j > L - Q + r - window if window > 0.  A row
+ * that sees nothing is zero; rows behind cu_q[n] are left as they are.  q, dst: [head_dim, n_head, rows]; k, v: [head_dim, n_head_kv, rows], F16 or
+ * BF16 (64 or 128 dims), strides multiples of 16 bytes.  q F32 / F16 / BF16 is rounded to k's type as in mi355x_flash_attn_ext, weights too; sums and
+ * softmax are F32; dst F32 / F16 / BF16.  Keys that a row does not see never reach it, whatever they hold.  max_q: an upper bound of the rows of
+ * one sequence as far as the caller knows it (0: unknown); it decides how the rows are cut, longer sequences are still complete. */
+typedef struct mi355x_attn_packed_desc {
+    mi355x_tensor   q, k, v, dst;  /* k, v: unused with a cache */
+    const int32_t * cu_q;          /* device [n+1] */
+    const int32_t * cu_k;          /* device [n+1] or NULL; unused with a cache */
+    const mi355x_kv_cache * cache; /* NULL: k and v */
+    const int32_t * seq;           /* device [n] or NULL, with a cache */
+    int32_t         n;
+    int32_t         causal;
+    int32_t         window;
+    int32_t         max_q;
+    float           scale;
+    int32_t         reserved;
+} mi355x_attn_packed_desc;
+MI355X_API int mi355x_attn_packed(mi355x_ctx * ctx, const mi355x_attn_packed_desc * d);
 
 /* ggml_norm (ggml/src/ggml.c:3139; CPU ggml-cpu/ops.cpp:3698-3765) with optional fused affine
  * (the ggml_mul + ggml_add that always follow it in whisper, src/whisper.cpp:2109-2114). */

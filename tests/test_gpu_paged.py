@@ -1,0 +1,535 @@
+"""The paged K/V cache, attention of one token over it and attention of packed prompts (mi355x_kv_*, mi355x_attn_paged, mi355x_attn_packed), through the C ABI.
+
+The cache's bookkeeping is compared exactly with a restatement in plain Python; the attentions with the definition in 64 bits.  Tolerances are worst-case
+bounds from the inputs of each case, with u(t) half a step of type t (f16 2^-11, bf16 2^-8, f32 2^-24):
+  * a score is a sum of D products in F32: off by at most e = (D + 8) * 2^-24 * scale * max_j sum_d |q_d k_jd| (and, where q is rounded to the cache's
+    type first, by u(cache) * scale * max_j sum_d |q_d k_jd| more), so a weight by the factor exp(2 e) (its own score and the maximum's), which in
+    the quotient counts twice: expm1(4 e);
+  * a weight rounded to the cache's type is off by u(cache); exp2 and the sums of L weights and products in F32 by (L + 32) * 2^-24 at most;
+  * all of these scale values of at most max|v|; the result is rounded to its own type: u(out) * |o|."""
+import ctypes as C
+import math
+import random
+
+import numpy as np
+import pytest
+
+from conftest import has_gpu
+
+pytestmark = pytest.mark.gpu
+
+U = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    import torch
+    assert torch.cuda.is_available(), "these tests need an MI355X"
+    from whisper_cpp_amd import kernels_api as ka
+    ctx = ka.Ctx(0)
+    yield ctx, ka, torch
+    ctx.close()
+
+
+def dt(torch, name):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+class Pool:
+    """A cache on the GPU and its restatement: lists of page numbers, and the keys that each sequence should hold"""
+
+    def __init__(self, gpu, n_seq=6, n_pages=40, max_pages=12, page=16, heads=2, dim=64, kind="f16", order="head", seed=0, fill=float("nan")):
+        self.ctx, self.ka, self.torch = gpu
+        torch = self.torch
+        self.page, self.heads, self.dim, self.kind, self.n_pages, self.max_pages = page, heads, dim, kind, n_pages, max_pages
+        shape = (n_pages, heads, page, dim) if order == "head" else (n_pages, page, heads, dim)
+        pool = [torch.full(shape, fill, dtype=dt(torch, kind), device="cuda") for _ in range(2)]      # memory that nothing has been written to yet: NaN
+        self.k, self.v = pool if order == "head" else [x.transpose(1, 2) for x in pool]
+        self.table = torch.full((n_seq, max_pages), 77, dtype=torch.int32, device="cuda")
+        self.len, self.ref = torch.full((n_seq,), 5, dtype=torch.int32, device="cuda"), torch.full((n_pages,), 9, dtype=torch.int32, device="cuda")
+        self.status = torch.full((1,), 64, dtype=torch.int32, device="cuda")
+        self.work = torch.empty(self.ka.kv_work_bytes(n_seq, n_pages), dtype=torch.uint8, device="cuda")
+        self.c = self.ka.kv_cache(self.k, self.v, self.table, self.len, self.ref, self.status, self.work)
+        torch.cuda.synchronize()
+        self.run(self.ctx.kv_reset_call(self.c))
+        self.gen = torch.Generator(device="cuda").manual_seed(seed)
+        # the restatement
+        self.rows, self.count = [[] for _ in range(n_seq)], [0] * n_pages
+        self.keys = [[] for _ in range(n_seq)]                       # of each sequence, key by key: (page written to, k, v) in 64 bits
+        self.content = {}                                            # (page, slot) -> (k [heads, dim], v), on the CPU in the cache's type
+
+    def run(self, call):
+        self.torch.cuda.synchronize()
+        call()
+        self.ctx.sync()
+
+    def ints(self, values):
+        return self.torch.tensor(values, dtype=self.torch.int32, device="cuda")
+
+    def append(self, entries, kind="f32", pad=0, layout="plain"):
+        """entries: [(sequence, rows)]; returns what the restatement expects of the status"""
+        torch = self.torch
+        n = sum(r for _, r in entries) + pad
+        k, v = (torch.randn(n, self.heads, self.dim, generator=self.gen, device="cuda").to(dt(torch, kind)) for _ in range(2))
+        if layout == "wide":                                         # rows of a larger projection: heads apart, rows further apart
+            k, v = (torch.cat([x, x], 2).repeat(1, 2, 1)[:, : self.heads, : self.dim] for x in (k, v))
+        cu = np.concatenate([[0], np.cumsum([r for _, r in entries])])
+        self.run(self.ctx.kv_append_call(self.c, self.ints([s for s, _ in entries]), self.ints(cu.tolist()), k, v))
+        return self._append(entries, k.to(dt(torch, self.kind)).cpu(), v.to(dt(torch, self.kind)).cpu(), cu)
+
+    def _append(self, entries, k, v, cu):
+        page, free, taken, todo = self.page, [p for p in range(self.n_pages) if self.count[p] == 0], 0, []
+        live = [s for s, _ in entries if s >= 0]
+        if any(s >= len(self.rows) for s in live) or len(set(live)) < len(live):
+            return self.ka.KV_BAD_ARG
+        for (s, r) in entries:
+            if s >= 0 and (len(self.keys[s]) + r) > self.max_pages * page:
+                return self.ka.KV_ROW_FULL
+        for i, (s, r) in enumerate(entries):
+            if s < 0:
+                continue
+            old = len(self.keys[s])
+            copy = r > 0 and old % page > 0 and self.count[self.rows[s][-1]] > 1
+            new = -(-(old + r) // page) - -(-old // page)
+            todo.append((i, s, r, old, copy, free[taken : taken + new + copy]))
+            taken += new + copy
+        if taken > len(free):
+            return self.ka.KV_OUT_OF_PAGES
+        for i, s, r, old, copy, pages in todo:
+            if copy:
+                was, now = self.rows[s][-1], pages.pop(0)
+                for j in range(old % page):
+                    self.content[now, j] = self.content[was, j]
+                self.count[was] -= 1
+                self.count[now] = 1
+                self.rows[s][-1] = now
+            for p in pages:
+                self.rows[s].append(p)
+                self.count[p] = 1
+            for j in range(r):
+                x = (k[cu[i] + j], v[cu[i] + j])
+                self.content[self.rows[s][(old + j) // page], (old + j) % page] = x
+                self.keys[s].append(x)
+        return 0
+
+    def truncate(self, entries):
+        self.run(self.ctx.kv_truncate_call(self.c, self.ints([s for s, _ in entries]), self.ints([x for _, x in entries])))
+        for s, keep in entries:
+            if 0 <= s < len(self.rows) and keep >= 0:
+                self.keys[s] = self.keys[s][:keep]
+                for p in self.rows[s][-(-len(self.keys[s]) // self.page) :]:
+                    self.count[p] -= 1
+                self.rows[s] = self.rows[s][: -(-len(self.keys[s]) // self.page)]
+
+    def fork(self, pairs):
+        self.run(self.ctx.kv_fork_call(self.c, self.ints([s for s, _ in pairs]), self.ints([d for _, d in pairs])))
+        before = [list(r) for r in self.rows], [list(x) for x in self.keys]
+        for s, d in pairs:
+            if d >= 0:
+                self.rows[d], self.keys[d] = (list(before[0][s]), list(before[1][s])) if s >= 0 else ([], [])
+        self.count = [sum(p in r for r in self.rows) for p in range(self.n_pages)]
+
+    def check(self, status=0, contents=True):
+        torch = self.torch
+        torch.cuda.synchronize()
+        want = [r + [-1] * (self.max_pages - len(r)) for r in self.rows]
+        assert int(self.status) == status
+        assert self.len.tolist() == [len(x) for x in self.keys]
+        assert self.table.tolist() == want
+        assert self.ref.tolist() == self.count
+        if contents:                                                 # every key where it belongs, and nothing anywhere else
+            for pool, which in ((self.k, 0), (self.v, 1)):
+                got = pool.cpu()
+                held = torch.zeros(self.n_pages, self.page, dtype=torch.bool)
+                for s, x in enumerate(self.keys):
+                    for j, kv in enumerate(x):
+                        p, slot = self.rows[s][j // self.page], j % self.page
+                        held[p, slot] = True
+                        assert torch.equal(got[p, :, slot], kv[which]), (s, j)
+                written = torch.zeros_like(held)
+                for p, slot in self.content:
+                    written[p, slot] = True
+                assert got.transpose(1, 2)[~written].isnan().all()   # slots that no call named are as they were
+        self.status.zero_()
+
+
+# ---- the cache ----------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind,io,order,dim,heads,page", [("f16", "f32", "head", 64, 3, 16), ("bf16", "f32", "key", 128, 2, 8), ("f16", "f16", "key", 64, 5, 1),
+                                                          ("bf16", "bf16", "head", 128, 1, 64), ("f16", "bf16", "head", 64, 2, 4), ("bf16", "f16", "key", 64, 20, 32)])
+def test_append_truncate_and_fork_keep_table_counts_and_keys_as_restated(gpu, kind, io, order, dim, heads, page):
+    p = Pool(gpu, page=page, heads=heads, dim=dim, kind=kind, order=order)
+    p.check()
+    assert p.append([(0, 3 * page - 1), (2, 0), (4, 1)], io) == 0
+    p.check()
+    assert p.append([(4, 2), (-1, 5), (1, page), (0, 2)], io, pad=3, layout="wide") == 0       # a row of padding, rows behind the last entry, a strided input
+    p.check()
+    p.fork([(0, 3), (4, 5), (4, 2), (-1, 1)])                        # shared pages; row 1 emptied
+    p.check()
+    assert p.append([(3, 1), (0, 2), (5, 1)], io) == 0               # sequences that share a partly filled page go their own ways
+    p.check()
+    p.fork([(3, 0), (0, 3), (2, 2), (5, -1)])                        # rows change places; one onto itself
+    p.check()
+    p.truncate([(0, page + 1), (3, 0), (5, 100), (-1, 0)])
+    p.check()
+    p.truncate([(0, 3), (0, 1), (0, 2)])                             # one sequence three times: the smallest holds
+    p.check()
+    assert p.append([(3, 2 * page + 1), (0, page)], io) == 0         # pages given back are taken again, lowest first
+    p.check()
+
+
+def test_many_rows_and_many_sequences_at_once(gpu):
+    rng = random.Random(3)
+    n = 1500                                                         # more entries than threads of the workgroup that hands pages out
+    p = Pool(gpu, n_seq=n, n_pages=9000, max_pages=5, page=4, heads=1, dim=64)
+    order = rng.sample(range(n), n)
+    assert p.append([(s, rng.randint(0, 9)) for s in order], "f16") == 0
+    p.check(contents=False)
+    pairs = [(s, d) for s, d in zip(rng.sample(range(n), n), rng.sample(range(n), n))]
+    p.fork(pairs)
+    p.check(contents=False)
+    assert p.append([(s, rng.randint(0, 5)) for s in order], "f16") == 0
+    p.check()
+
+
+def test_a_call_that_cannot_be_done_says_why_and_changes_nothing(gpu):
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_pages=10, max_pages=6, page=4)
+    assert p.append([(0, 9), (1, 4)]) == 0
+    p.check()
+    assert p.append([(2, 1), (3, 24)]) == ka.KV_OUT_OF_PAGES         # 4 pages are held, 7 more wanted, 6 free: not even entry 0 is done
+    p.check(ka.KV_OUT_OF_PAGES)
+    assert p.append([(2, 1), (0, 16)]) == ka.KV_ROW_FULL
+    p.check(ka.KV_ROW_FULL)
+    assert p.append([(2, 1), (2, 1)]) == ka.KV_BAD_ARG
+    p.check(ka.KV_BAD_ARG)
+    assert p.append([(2, 1), (6, 1)]) == ka.KV_BAD_ARG
+    p.check(ka.KV_BAD_ARG)
+    k = torch.randn(4, 2, 64, device="cuda")
+    for cu in ([0, 3, 2], [0, 2, 5], [-1, 1, 2]):                    # offsets that fall, leave the rows, start before them
+        p.run(ctx.kv_append_call(p.c, p.ints([2, 3]), p.ints(cu), k, k))
+        p.check(ka.KV_BAD_ARG)
+    for src, dst in (([0, 1], [2, 2]), ([0, 6], [2, 3]), ([0, 1], [2, 6])):
+        p.run(ctx.kv_fork_call(p.c, p.ints(src), p.ints(dst)))
+        p.check(ka.KV_BAD_ARG)
+    p.run(ctx.kv_truncate_call(p.c, p.ints([6, 0]), p.ints([0, -1])))
+    p.check(ka.KV_BAD_ARG)
+    assert p.append([(2, 24)]) == 0                                  # the last free page is used up ...
+    p.check()
+    assert p.append([(0, 0), (1, 0)]) == 0                           # ... and calls without a need go on working
+    p.check()
+
+
+@pytest.mark.parametrize("order,order2,dim,page", [("head", "head", 64, 16), ("key", "head", 128, 4), ("head", "key", 64, 1)])
+def test_compact_moves_the_held_pages_and_renames_them(gpu, order, order2, dim, page):
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_pages=60, page=page, dim=dim, order=order, heads=3)
+    for i in range(3):
+        assert p.append([(s, 2 * page - s % 2) for s in range(6)]) == 0
+        p.truncate([(i, 0)])
+    p.fork([(4, 0), (5, 1)])
+    assert p.append([(0, 1), (4, 1)]) == 0
+    p.check()
+    used = [x for x in range(60) if p.count[x]]
+    for n_pages, wide in ((len(used), 0), (len(used) + 7, 3), (len(used) - 1, 0)):
+        q = Pool(gpu, n_pages=n_pages, max_pages=12 + wide, page=page, dim=dim, order=order2, heads=3)
+        p.run(ctx.kv_compact_call(p.c, q.c))
+        p.check()                                                    # the old cache is as it was
+        if n_pages < len(used):
+            q.check(ka.KV_OUT_OF_PAGES)                              # the new one too, and says why
+            continue
+        name = {x: i for i, x in enumerate(used)}
+        q.rows, q.keys = [[name[x] for x in r] for r in p.rows], [list(x) for x in p.keys]
+        q.count = [p.count[x] for x in used] + [0] * (n_pages - len(used))
+        q.content = {(i, j): None for i in range(len(used)) for j in range(page)}            # whole pages move, unused slots among them
+        q.check()
+        full = 0 if n_pages > len(used) else ka.KV_OUT_OF_PAGES
+        assert q.append([(2, 1), (0, 2)]) == full                    # and it is a cache to go on with, if it has room
+        q.check(full)
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------
+
+
+def expect(torch, q, k, v, see, scale, kind, q_kind, out_kind, round_q, round_w):
+    """(64-bit result, allowed error) of rows q [H, D] over k, v [L, Hkv, D]; see [L]"""
+    H, D = q.shape
+    G = H // k.shape[1]
+    q, k, v = q.double(), k.double()[see], v.double()[see]
+    if len(k) == 0:
+        return torch.zeros(H, D, dtype=torch.float64), torch.zeros(H, D, dtype=torch.float64)
+    k, v = k.repeat_interleave(G, 1), v.repeat_interleave(G, 1)      # [L, H, D]
+    x = torch.einsum("hd,lhd->hl", q, k) * scale
+    w = torch.softmax(x, 1)
+    o = torch.einsum("hl,lhd->hd", w, v)
+    size = (torch.einsum("hd,lhd->hl", q.abs(), k.abs()) * abs(scale)).amax(1)
+    e = size * ((D + 8) * U["f32"] + (U[kind] if round_q else 0.0))
+    per = torch.expm1(4 * e) + (2 * U[kind] if round_w else 0.0) + (len(k) + 32) * U["f32"]
+    return o, per[:, None] * v.abs().amax(0) .amax(-1, keepdim=True) + U[out_kind] * o.abs() + 1e-30
+
+
+def same(torch, got, o, tol):
+    got = got.double().cpu()
+    for f in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(f(got), f(o)), (f.__name__, int(f(got).sum()), int(f(o).sum()), o.numel())
+    fine = o.isfinite()
+    off = ((got - o).abs() - tol)[fine]
+    assert off.numel() == 0 or float(off.max()) <= 0, (float((got - o).abs()[fine].max()), float(off.max()))
+
+
+LENGTHS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 255, 257, 300]
+
+
+@pytest.mark.parametrize("kind,q_kind,out_kind", [("f16", "f32", "f32"), ("bf16", "f32", "f32"), ("f16", "f16", "f16"), ("bf16", "bf16", "bf16"), ("bf16", "f16", "f32"), ("f16", "f16", "bf16")])
+@pytest.mark.parametrize("dim,kv_heads,heads,page,order,window", [(64, 2, 2, 16, "head", 0), (128, 2, 8, 32, "key", 0), (64, 1, 7, 1, "key", 40), (128, 1, 20, 8, "head", 33), (64, 3, 48, 64, "head", 1),
+                                                                  (128, 4, 4, 128, "key", 500)])
+def test_attention_of_one_token(gpu, kind, q_kind, out_kind, dim, kv_heads, heads, page, order, window):
+    """every length around tile, page and window borders, an order of sequences of the caller's, an entry of -1, pages with NaN behind the sequences' ends"""
+    ctx, ka, torch = gpu
+    rng = random.Random(dim + heads + page)
+    need = sum(-(-x // page) for x in LENGTHS) + 5
+    p = Pool(gpu, n_seq=len(LENGTHS), n_pages=need, max_pages=-(-300 // page), page=page, heads=kv_heads, dim=dim, kind=kind, order=order)
+    lens = list(LENGTHS)
+    rng.shuffle(lens)
+    assert p.append([(s, x) for s, x in enumerate(lens)], kind) == 0
+    seq = rng.sample(range(len(lens)), len(lens)) + [-1, 3]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(len(seq), heads, dim, generator=gen, device="cuda").mul_(2).to(dt(torch, q_kind))
+    scale = 1 / math.sqrt(dim)
+    for max_len in (0, 300, 1):                                      # what the caller says of the lengths never changes what is computed
+        out = torch.full((len(seq), heads, dim), 7.0, device="cuda").to(dt(torch, out_kind))
+        work = torch.empty(max(16, ka.attn_paged_work_bytes(p.c, len(seq), heads, max_len)), dtype=torch.uint8, device="cuda")
+        p.run(ctx.attn_paged_call(p.c, q, out, seq=p.ints(seq), scale=scale, window=window, max_len=max_len, work=work))
+        p.check(contents=False)
+        for i, s in enumerate(seq):
+            keys = p.keys[s] if s >= 0 else []
+            k, v = (torch.stack([x[w] for x in keys]) if keys else torch.zeros(0, kv_heads, dim) for w in (0, 1))
+            see = torch.arange(len(keys)) >= (len(keys) - window if window else 0)
+            o, tol = expect(torch, q[i].cpu(), k, v, see, scale, kind, q_kind, out_kind, False, q_kind == kind)
+            same(torch, out[i], o, tol)
+
+
+@pytest.mark.parametrize("n,length,kv_heads,heads,dim,kind", [(1, 5003, 1, 1, 64, "f16"), (2, 40001, 2, 8, 128, "bf16"), (5, 3001, 8, 64, 128, "f16")])
+def test_attention_of_one_token_split_over_a_long_cache_and_joined(gpu, n, length, kv_heads, heads, dim, kind):
+    ctx, ka, torch = gpu
+    page, gen = 32, torch.Generator(device="cuda").manual_seed(4)
+    lens = [length, 0, 1, length // 2, 700][:n]
+    held = [-(-x // page) for x in lens]
+    k, v = (torch.randn(sum(held), kv_heads, page, dim, generator=gen, device="cuda").to(dt(torch, kind)) for _ in range(2))
+    pages = torch.randperm(sum(held), generator=torch.Generator().manual_seed(1)).int()
+    table = torch.full((n, max(held)), -1, dtype=torch.int32)
+    at = 0
+    for s, h in enumerate(held):
+        table[s, :h] = pages[at : at + h]
+        at += h
+    zero = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+    work, status, dtab, dlen, ref = torch.empty(ka.kv_work_bytes(n, sum(held)), dtype=torch.uint8, device="cuda"), zero(1), table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), zero(sum(held))
+    c = ka.kv_cache(k, v, dtab, dlen, ref, status, work)
+    q = torch.randn(n, heads, dim, generator=gen, device="cuda")
+    q[0] *= 6                                                        # a few keys far above the others: weights over many powers of two
+    scale, rows = 1 / math.sqrt(dim), []
+    space = torch.empty(ka.attn_paged_work_bytes(c, n, heads, length), dtype=torch.uint8, device="cuda")
+    assert space.numel() > 0
+    for rep in range(2):
+        out = torch.full_like(q, 3.0)
+        torch.cuda.synchronize()
+        ctx.attn_paged_call(c, q, out, scale=scale, max_len=length, work=space)()
+        ctx.sync()
+        rows.append(out)
+    assert torch.equal(rows[0], rows[1])                             # nothing depends on which share ends first
+    for s in range(n):
+        flat = [x.cpu()[table[s, : held[s]].long()].transpose(1, 2).reshape(-1, kv_heads, dim)[: lens[s]] for x in (k, v)]
+        o, tol = expect(torch, q[s].cpu(), *flat, torch.ones(lens[s], dtype=torch.bool), scale, kind, "f32", "f32", False, False)
+        same(torch, rows[0][s], o, tol)
+
+
+def packed_case(gpu, kind, q_kind, out_kind, dim, kv_heads, heads, q_lens, k_lens=None, window=0, causal=True, page=0, order="head", spoil=None, max_q=0, scale=None):
+    """one call of the packed attention over rows of its own (page 0) or over a cache, against the definition.  `spoil`: {(sequence, key): (k, v)}"""
+    ctx, ka, torch = gpu
+    gen, n = torch.Generator(device="cuda").manual_seed(9), len(q_lens)
+    ks = k_lens or q_lens
+    cu = np.concatenate([[0], np.cumsum(q_lens)]).tolist()
+    scale = 1 / math.sqrt(dim) if scale is None else scale
+    q = torch.randn(cu[-1] + 2, heads, dim, generator=gen, device="cuda").mul_(2).to(dt(torch, q_kind))
+    out = torch.full((cu[-1] + 2, heads, dim), 7.0, device="cuda").to(dt(torch, out_kind))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    if page:
+        p = Pool(gpu, n_seq=n + 1, n_pages=sum(-(-x // page) for x in ks) + 2, max_pages=max(-(-x // page) for x in ks) + 1, page=page, heads=kv_heads, dim=dim, kind=kind, order=order)
+        row = random.Random(2).sample(range(n + 1), n)
+        assert p.append([(row[i], ks[i]) for i in range(n)], kind) == 0
+        kv = [[torch.stack([x[w] for x in p.keys[r]]) if p.keys[r] else torch.zeros(0, kv_heads, dim) for w in (0, 1)] for r in row]
+        for (s, j), (a, b) in (spoil or {}).items():
+            at = p.rows[row[s]][j // page], slice(None), j % page
+            p.k[at], p.v[at] = a, b
+            kv[s][0][j], kv[s][1][j] = a, b
+        call = ctx.attn_packed_call(q, out, ints(cu), cache=p.c, seq=ints(row), scale=scale, causal=causal, window=window, max_q=max_q)
+    else:
+        ck = np.concatenate([[0], np.cumsum(ks)]).tolist()
+        k, v = (torch.randn(ck[-1] + 1, kv_heads, 2 * dim if order == "key" else dim, generator=gen, device="cuda").to(dt(torch, kind))[..., :dim] for _ in range(2))
+        for (s, j), (a, b) in (spoil or {}).items():
+            k[ck[s] + j], v[ck[s] + j] = a, b
+        k[ck[-1]:], v[ck[-1]:] = float("nan"), float("nan")
+        kv = [[x[ck[i] : ck[i + 1]].cpu() for x in (k, v)] for i in range(n)]
+        call = ctx.attn_packed_call(q, out, ints(cu), k=k, v=v, cu_k=ints(ck) if k_lens else None, scale=scale, causal=causal, window=window, max_q=max_q)
+    torch.cuda.synchronize()
+    call()
+    ctx.sync()
+    assert torch.equal(out[cu[-1] :].float(), torch.full_like(out[cu[-1] :], 7.0).float())       # rows behind the last sequence
+    for i in range(n):
+        L, Q = ks[i], q_lens[i]
+        rows = range(Q) if Q < 40 else sorted(set(list(range(6)) + list(range(Q - 6, Q)) + random.Random(i).sample(range(Q), 12)))
+        for r in rows:
+            j = torch.arange(L)
+            see = j <= L - Q + r if causal else j >= 0
+            if window:
+                see = see & (j > L - Q + r - window)
+            o, tol = expect(torch, q[cu[i] + r].cpu(), kv[i][0], kv[i][1], see, scale, kind, q_kind, out_kind, q_kind != kind, True)
+            try:
+                same(torch, out[cu[i] + r], o, tol)
+            except AssertionError as e:
+                raise AssertionError(f"sequence {i} row {r} of {Q}, {L} keys: {e}")
+
+
+@pytest.mark.parametrize("kind,q_kind,out_kind", [("f16", "f16", "f16"), ("bf16", "bf16", "bf16"), ("f16", "f32", "f32"), ("bf16", "f16", "f32")])
+@pytest.mark.parametrize("dim,kv_heads,heads,window,order", [(64, 2, 2, 0, "head"), (128, 1, 4, 0, "key"), (64, 1, 3, 20, "head"), (128, 2, 14, 100, "head"), (64, 1, 128, 0, "head")])
+def test_attention_of_packed_prompts(gpu, kind, q_kind, out_kind, dim, kv_heads, heads, window, order):
+    packed_case(gpu, kind, q_kind, out_kind, dim, kv_heads, heads, [1, 0, 5, 64, 17, 130, 63, 0, 257], window=window, order=order)
+
+
+@pytest.mark.parametrize("dim,kv_heads,heads,page,order,causal,window", [(64, 2, 4, 16, "head", True, 0), (128, 1, 8, 4, "key", True, 50), (128, 2, 2, 64, "head", True, 0), (64, 1, 5, 32, "key", False, 0),
+                                                                         (64, 2, 2, 8, "head", False, 30)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attention_of_prompt_pieces_over_the_cache(gpu, kind, dim, kv_heads, heads, page, order, causal, window):
+    """fewer rows than keys (the rest is the past), as many, more (the first rows see nothing), none of either"""
+    packed_case(gpu, kind, kind, kind, dim, kv_heads, heads, [3, 1, 70, 9, 0, 40, 4], [200, 1, 70, 3, 33, 0, 131], page=page, order=order, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("max_q", [0, 1, 12, 64, 4000])
+@pytest.mark.parametrize("dim,heads", [(64, 1), (128, 4)])
+def test_what_the_caller_says_of_the_rows_never_changes_what_is_computed(gpu, dim, heads, max_q):
+    packed_case(gpu, "f16", "f16", "f16", dim, 1, heads, [4, 1, 12, 70], [700, 1, 300, 70], max_q=max_q)
+    packed_case(gpu, "f16", "f16", "f16", dim, 1, heads, [4, 1, 12, 70], [700, 1, 300, 70], max_q=max_q, page=16)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("page,max_q", [(0, 0), (16, 0), (0, 8), (16, 8)])
+def test_infinities_and_nan_reach_only_the_rows_that_see_them(gpu, kind, page, max_q):
+    inf, nan = float("inf"), float("nan")
+    q = [100, 90] if max_q == 0 else [8, 5]
+    ks = [100, 90] if max_q == 0 else [108, 90]
+    late = ks[0] - 3                                                 # seen by the last three rows alone
+    packed_case(gpu, kind, kind, kind, 64, 1, 2, q, ks, page=page, max_q=max_q, spoil={(0, late): (0.5, nan), (1, ks[1] - 1): (0.25, inf)})
+    packed_case(gpu, kind, kind, kind, 128, 1, 1, q, ks, page=page, max_q=max_q, spoil={(0, late): (0.0, inf), (0, late + 1): (0.0, -inf), (1, ks[1] - 1): (nan, 1.0)})
+    packed_case(gpu, kind, kind, kind, 64, 2, 2, q, ks, page=page, max_q=max_q, window=2, spoil={(0, late - 2): (nan, nan), (1, ks[1] - 4): (1.0, -inf)})
+
+
+def test_the_largest_and_smallest_values_of_the_type(gpu):
+    """keys and values at the type's ends: scores of +-6e4 * |q| * scale do not overflow F32, one weight takes it all"""
+    ctx, ka, torch = gpu
+    top = {"f16": 65504.0, "bf16": 1e30}
+    for kind in ("f16", "bf16"):
+        p = Pool(gpu, n_seq=1, n_pages=4, max_pages=4, page=16, heads=1, dim=64, kind=kind)
+        assert p.append([(0, 40)], kind) == 0
+        k, v = (x.reshape(-1, 64)[:40] for x in (p.k, p.v))          # pages 0, 1, 2 in order
+        k[7], k[20], v[7], v[9] = top[kind] * 1e-3, -top[kind] * 1e-3, top[kind], 1e-7
+        q = torch.zeros(1, 1, 64, device="cuda")
+        q[..., 0] = 1.0
+        out = torch.empty(1, 1, 64, device="cuda")
+        p.run(ctx.attn_paged_call(p.c, q, out, scale=1.0))
+        assert torch.equal(out[0, 0], v[7].float())                  # exp of the runner-up underflows to nothing
+        q[..., 0] = -1.0
+        p.run(ctx.attn_paged_call(p.c, q, out, scale=1.0))
+        assert torch.equal(out[0, 0], v[20].float())
+        p.run(ctx.attn_paged_call(p.c, q, out, scale=0.0))           # equal weights
+        want = v.double().mean(0)
+        assert float(((out[0, 0].double() - want).abs() / want.abs().clamp_min(v.double().abs().mean(0) * 1e-2)).max()) < 100 * 40 * U["f32"]
+
+
+def test_a_decode_loop_captured_into_a_graph_and_replayed(gpu):
+    """append, attention, fork and truncate of a step captured once on the context's stream; every replay, with new lists and eager work of the program
+    between the replays, equals the same step run eagerly on a second cache"""
+    ctx, ka, torch = gpu
+    stream = torch.cuda.ExternalStream(ka.lib().mi355x_ctx_stream(ctx.h))
+    n, heads = 4, 2
+    caches = [Pool(gpu, n_seq=n, n_pages=64, max_pages=16, page=4, heads=heads, dim=64, seed=1) for _ in range(2)]
+    for p in caches:
+        assert p.append([(s, 5 + 7 * s) for s in range(n)]) == 0
+    seq, cu = caches[0].ints(list(range(n))), caches[0].ints(list(range(n + 1)))
+    k, v, q = (torch.zeros(n, heads, 64, device="cuda") for _ in range(3))
+    src, dst, keep = caches[0].ints([0] * n), caches[0].ints(list(range(n))), caches[0].ints([1000] * n)
+    outs, steps = [torch.zeros(n, heads, 64, device="cuda") for _ in caches], []
+    for p, out in zip(caches, outs):
+        work = torch.empty(max(16, ka.attn_paged_work_bytes(p.c, n, heads)), dtype=torch.uint8, device="cuda")
+        steps.append([ctx.kv_append_call(p.c, seq, cu, k, v), ctx.attn_paged_call(p.c, q, out, scale=0.125, work=work), ctx.kv_fork_call(p.c, src, dst), ctx.kv_truncate_call(p.c, seq, keep)])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for call in steps[1]:
+            call()
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    rng = random.Random(8)
+    for rep in range(6):
+        for x in (k, v, q):
+            x.copy_(torch.randn(n, heads, 64, generator=gen, device="cuda"))
+        src.copy_(caches[0].ints([rng.randrange(n) for _ in range(n)]))
+        keep.copy_(caches[0].ints([rng.choice((1000, 3, 9)) for _ in range(n)]))
+        torch.cuda.synchronize()
+        for call in steps[0]:
+            call()
+        ctx.sync()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1])
+        for x in ("table", "len", "ref", "status"):
+            assert torch.equal(getattr(caches[0], x), getattr(caches[1], x)), (rep, x)
+        assert int(caches[0].status) == 0
+
+
+@pytest.mark.parametrize("kind,dim,kv_heads,heads,page", [("f16", 64, 2, 4, 16), ("bf16", 128, 1, 4, 8)])
+def test_serving_streams_from_prompt_to_beams(gpu, kind, dim, kv_heads, heads, page):
+    """prompts into the cache and attention over them, a second piece of each over the cache, single tokens with forks between them, a compaction in
+    the middle: every result equals attention over the keys that the restatement holds"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=6, n_pages=120, max_pages=20, page=page, heads=kv_heads, dim=dim, kind=kind)
+    scale, gen, rng = 1 / math.sqrt(dim), torch.Generator(device="cuda").manual_seed(3), random.Random(3)
+
+    def queries(rows):
+        return torch.randn(rows, heads, dim, generator=gen, device="cuda").to(dt(torch, kind))
+
+    def hold(out, q, i, s, last):
+        k, v = (torch.stack([x[w] for x in p.keys[s]]) for w in (0, 1))
+        o, tol = expect(torch, q[i].cpu(), k, v, torch.arange(len(k)) <= last, scale, kind, kind, kind, False, True)
+        same(torch, out[i], o, tol)
+
+    for piece in ([7, 0, 33], [20, 2, 1]):                           # the prompts in two pieces
+        assert p.append(list(enumerate(piece)), kind) == 0
+        q, cu = queries(sum(piece)), np.concatenate([[0], np.cumsum(piece)]).tolist()
+        out = torch.zeros_like(q)
+        p.run(ctx.attn_packed_call(q, out, p.ints(cu), cache=p.c, seq=p.ints([0, 1, 2]), scale=scale))
+        for s, x in enumerate(piece):
+            for r in range(x):
+                hold(out, q, cu[s] + r, s, len(p.keys[s]) - x + r)
+    p.fork([(0, 3), (2, 4), (2, 5)])
+    for step in range(10):
+        live = [0, 2, 3, 4, 5]
+        assert p.append([(s, 1) for s in live], kind) == 0
+        q = queries(len(live))
+        out = torch.zeros_like(q)
+        work = torch.empty(max(16, ka.attn_paged_work_bytes(p.c, len(live), heads)), dtype=torch.uint8, device="cuda")
+        p.run(ctx.attn_paged_call(p.c, q, out, seq=p.ints(live), scale=scale, work=work))
+        p.check(contents=False)
+        for i, s in enumerate(live):
+            hold(out, q, i, s, len(p.keys[s]) - 1)
+        p.fork([(rng.choice((2, 4, 5)), d) for d in (2, 4, 5)])
+        if step == 5:
+            other = Pool(gpu, n_seq=6, n_pages=90, max_pages=20, page=page, heads=kv_heads, dim=dim, kind=kind, order="key", seed=5)
+            p.run(ctx.kv_compact_call(p.c, other.c))
+            used = [x for x in range(p.n_pages) if p.count[x]]
+            name = {x: i for i, x in enumerate(used)}
+            other.rows, other.keys = [[name[x] for x in r] for r in p.rows], p.keys
+            other.count = [p.count[x] for x in used] + [0] * (90 - len(used))
+            other.content = {(name[a], b): x for (a, b), x in p.content.items() if a in name}
+            p = other
+            p.check(contents=False)
+    p.check(contents=False)

@@ -1,0 +1,133 @@
+"""What the calls of the paged cache and its attentions refuse (include/mi355x_kernels.h: mi355x_kv_*, mi355x_attn_paged, mi355x_attn_packed): checked on the
+host before anything is launched, so without a device.  The context of a refused call is never touched: a blank block stands for it."""
+import ctypes as C
+
+import pytest
+
+from whisper_cpp_amd import kernels_api as ka
+
+BLANK = C.create_string_buffer(65536)
+CTX = C.cast(BLANK, C.c_void_p)
+MEM = (C.c_char * 4096).from_buffer(bytearray(4096))
+AT = (C.addressof(MEM) + 63) // 64 * 64
+
+
+def cache(**change):
+    c = ka.KvCache()
+    c.k, c.v, c.type, c.head_dim, c.n_head_kv, c.page_size, c.n_pages, c.n_seq, c.max_pages = AT, AT, ka.F16, 64, 2, 16, 8, 4, 4
+    c.nb_key, c.nb_head, c.nb_page = 128, 2048, 4096
+    c.table = c.len = c.ref = c.status = c.work = AT
+    for name, value in change.items():
+        setattr(c, name, value)
+    return c
+
+
+def rows(n=3, heads=2, dim=64, kind=ka.F32, at=AT, nb=None):
+    size = 4 if kind == ka.F32 else 2
+    return ka.tensor(at, kind, [dim, heads, n], nb or [size, size * dim, size * dim * heads])
+
+
+def refused(name, *args):
+    assert getattr(ka.lib(), name)(CTX, *args) == -1
+    assert ka.lib().mi355x_last_error()
+
+
+BAD_CACHES = [dict(k=None), dict(v=None), dict(table=None), dict(len=None), dict(ref=None), dict(status=None), dict(work=None), dict(type=ka.F32), dict(type=ka.Q8_0), dict(head_dim=80),
+              dict(head_dim=0), dict(n_head_kv=0), dict(n_head_kv=513), dict(page_size=0), dict(page_size=24), dict(page_size=8192), dict(n_pages=0), dict(n_seq=0), dict(n_seq=300000),
+              dict(max_pages=0), dict(max_pages=1 << 27), dict(nb_key=120), dict(nb_key=64), dict(nb_head=8), dict(nb_page=0), dict(k=AT + 8), dict(table=AT + 2), dict(nb_page=-4096)]
+
+
+@pytest.mark.parametrize("change", BAD_CACHES, ids=lambda d: "-".join(f"{k}={v}" for k, v in d.items()))
+def test_every_call_refuses_a_cache_that_does_not_fit(change):
+    c, t = cache(**change), rows()
+    d = ka.AttnPagedDesc()
+    d.q, d.dst, d.scale = rows(4), rows(4), 1.0
+    p = ka.AttnPackedDesc()
+    p.q, p.dst, p.cu_q, p.cache, p.n = rows(), rows(), AT, C.pointer(c), 1
+    refused("mi355x_kv_reset", C.byref(c))
+    refused("mi355x_kv_append", C.byref(c), 1, AT, AT, C.byref(t), C.byref(t))
+    refused("mi355x_kv_truncate", C.byref(c), 1, AT, AT)
+    refused("mi355x_kv_fork", C.byref(c), 1, AT, AT)
+    refused("mi355x_kv_compact", C.byref(c), C.byref(cache(k=AT + 1024, v=AT + 2048)))
+    refused("mi355x_kv_compact", C.byref(cache(k=AT + 1024, v=AT + 2048)), C.byref(c))
+    refused("mi355x_attn_paged", C.byref(c), C.byref(d))
+    refused("mi355x_attn_packed", C.byref(p))
+
+
+def test_lists_and_rows_that_do_not_fit_are_refused():
+    c = cache()
+    ok, cases = rows(), [rows(dim=128), rows(heads=3), rows(at=AT + 4), rows(kind=ka.I32), rows(nb=[4, 250, 512]), rows(nb=[8, 512, 1024]), rows(n=4), rows(kind=ka.F16), rows(at=None)]
+    for t in cases:
+        refused("mi355x_kv_append", C.byref(c), 1, AT, AT, C.byref(ok), C.byref(t))
+    refused("mi355x_kv_append", C.byref(c), 1, AT, AT, None, C.byref(ok))
+    refused("mi355x_kv_append", C.byref(c), 5, AT, AT, C.byref(ok), C.byref(ok))
+    refused("mi355x_kv_append", C.byref(c), -1, AT, AT, C.byref(ok), C.byref(ok))
+    refused("mi355x_kv_append", C.byref(c), 1, None, AT, C.byref(ok), C.byref(ok))
+    refused("mi355x_kv_append", C.byref(c), 1, AT, AT + 1, C.byref(ok), C.byref(ok))
+    refused("mi355x_kv_truncate", C.byref(c), 1, AT, None)
+    refused("mi355x_kv_truncate", C.byref(c), -1, AT, AT)
+    refused("mi355x_kv_fork", C.byref(c), 1, None, AT)
+    refused("mi355x_kv_fork", C.byref(c), 8193, AT, AT)
+    other = dict(k=AT + 1024, v=AT + 2048, table=AT + 64, len=AT + 128, ref=AT + 192, work=AT + 256)
+    for change in (dict(type=ka.BF16), dict(head_dim=128, nb_key=256), dict(n_head_kv=1), dict(page_size=8), dict(n_seq=5), dict(max_pages=3), dict(k=AT), dict(table=AT), dict(work=AT)):
+        refused("mi355x_kv_compact", C.byref(c), C.byref(cache(**{**other, **change})))
+
+
+def test_attention_of_one_token_refuses_what_it_cannot_do():
+    c = cache(max_pages=4096)
+    for change in (dict(q=rows(heads=3)), dict(q=rows(dim=128)), dict(dst=rows(4)), dict(dst=rows(kind=ka.Q8_0)), dict(q=rows(5), dst=rows(5)), dict(window=-1), dict(max_len=-1), dict(seq=AT + 2),
+                   dict(work=None), dict(work=AT + 4), dict(work_bytes=64)):
+        d = ka.AttnPagedDesc()
+        d.q, d.dst, d.scale, d.work, d.work_bytes = rows(), rows(), 1.0, AT, 1 << 30
+        for name, value in change.items():
+            setattr(d, name, value)
+        refused("mi355x_attn_paged", C.byref(c), C.byref(d))
+    refused("mi355x_attn_paged", C.byref(c), None)
+    assert ka.attn_paged_work_bytes(c, 3, 2) > 64                    # 65536 keys: split, so the work area is wanted
+    assert ka.attn_paged_work_bytes(c, 3, 2, 100) == 0               # at most 100: not
+    assert ka.attn_paged_work_bytes(c, 3, 3) == 0 and ka.attn_paged_work_bytes(c, 0, 2) == 0
+    assert ka.kv_work_bytes(4, 8) > 0 and ka.kv_work_bytes(0, 8) == 0 and ka.kv_work_bytes(4, -1) == 0
+
+
+def test_attention_of_packed_rows_refuses_what_it_cannot_do():
+    kv = rows(kind=ka.F16)
+    for change in (dict(q=rows(heads=3)), dict(q=rows(dim=128)), dict(q=rows(heads=258)), dict(dst=rows(4)), dict(k=rows()), dict(v=rows(kind=ka.BF16)), dict(v=rows(2, kind=ka.F16)), dict(k=rows(dim=80, kind=ka.F16)),
+                   dict(v=rows(kind=ka.F16, nb=[2, 128, 512])), dict(cu_q=None), dict(cu_q=AT + 2), dict(cu_k=AT + 2), dict(n=-1), dict(window=-1), dict(max_q=-1), dict(q=rows(at=AT + 8))):
+        d = ka.AttnPackedDesc()
+        d.q, d.k, d.v, d.dst, d.cu_q, d.n, d.scale = rows(), kv, kv, rows(), AT, 1, 1.0
+        for name, value in change.items():
+            setattr(d, name, value)
+        refused("mi355x_attn_packed", C.byref(d))
+    d.cache, d.cu_q, d.n, d.max_q, d.q = C.pointer(cache()), AT, 5, 0, rows()
+    refused("mi355x_attn_packed", C.byref(d))                        # more entries than the cache has sequences, and no list of them
+    refused("mi355x_attn_packed", None)
+
+
+def test_python_descriptions_refuse_arrays_that_do_not_fit():
+    import torch
+    k = torch.zeros(8, 2, 16, 64, dtype=torch.float16)
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32)  # noqa: E731
+    ok = dict(k=k, v=k.clone(), table=i(4, 4), length=i(4), ref=i(8), status=i(1), work=torch.zeros(ka.kv_work_bytes(4, 8), dtype=torch.uint8))
+    c = ka.kv_cache(**ok)
+    assert (c.n_pages, c.n_head_kv, c.page_size, c.head_dim, c.n_seq, c.max_pages, c.nb_key, c.nb_head, c.nb_page) == (8, 2, 16, 64, 4, 4, 128, 2048, 4096)
+    t = ka.kv_cache(**{**ok, "k": k.transpose(1, 2).contiguous().transpose(1, 2), "v": k.transpose(1, 2).contiguous().transpose(1, 2)})
+    assert (t.nb_key, t.nb_head) == (256, 128)
+    for change in (dict(v=k[:7]), dict(v=k.float()), dict(table=i(4)), dict(table=i(4, 4).long()), dict(length=i(3)), dict(ref=i(7)), dict(work=i(3)), dict(k=k.double(), v=k.double()), dict(table=i(8, 4)[::2])):
+        with pytest.raises(ValueError):
+            ka.kv_cache(**{**ok, **change})
+
+
+def test_ctypes_mirrors_of_the_paged_structs(tmp_path):
+    import subprocess
+    from conftest import ROOT
+    probes = {"mi355x_kv_cache": ka.KvCache, "mi355x_attn_paged_desc": ka.AttnPagedDesc, "mi355x_attn_packed_desc": ka.AttnPackedDesc}
+    src = ["#include <stdio.h>", "#include <stddef.h>", '#include "mi355x_kernels.h"', "int main(void) {"]
+    for s, m in probes.items():
+        src.append(f'  printf("{s} %zu", sizeof({s}));')
+        src += [f'  printf(" %zu", offsetof({s}, {f[0]}));' for f in m._fields_] + ['  printf("\\n");']
+    (tmp_path / "layout.c").write_text("\n".join(src + ["  return 0;", "}"]))
+    subprocess.run(["gcc", f"-I{ROOT / 'include'}", str(tmp_path / "layout.c"), "-o", str(tmp_path / "layout")], check=True)
+    for line in subprocess.run([str(tmp_path / "layout")], check=True, stdout=subprocess.PIPE, text=True).stdout.strip().splitlines():
+        name, size, *offs = line.split()
+        assert C.sizeof(probes[name]) == int(size)
+        assert [getattr(probes[name], f[0]).offset for f in probes[name]._fields_] == [int(x) for x in offs]

@@ -22,7 +22,7 @@ BUILD = ROOT / "build"
 REF = Path(os.environ.get("WHISPER_REF", "/root/reference"))
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
-KERNEL_SRCS = ["ctx.hip", "elementwise.hip", "gemv.hip", "decode.hip", "decode_q.hip", "decode_mx.hip", "gemm_mfma.hip", "fattn.hip", "fattn_exact.hip", "mel.hip", "mul_mat.hip", "mmq.hip"]
+KERNEL_SRCS = ["ctx.hip", "elementwise.hip", "gemv.hip", "decode.hip", "decode_q.hip", "decode_mx.hip", "gemm_mfma.hip", "fattn.hip", "fattn_exact.hip", "mel.hip", "mul_mat.hip", "mmq.hip", "kv_cache.hip", "attn_paged.hip", "attn_packed.hip"]
 BACKEND_SRCS = ["ggml_mi355x.cpp", "mi_buffers.cpp", "mi_planner.cpp", "mi_batching.cpp", "mi_distribution.cpp"]      # one internal header: mi_backend.h
 
 # no packed FP32 (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this hardware (the host pass warns that it does not know the feature)
@@ -53,7 +53,7 @@ def _stale(out: Path, deps):
 def build_kernels(verbose=False):
     LIB.mkdir(exist_ok=True)
     (BUILD / "kernels").mkdir(parents=True, exist_ok=True)
-    hdrs = [CSRC / "kernels" / "common.h", CSRC / "kernels" / "decode_common.h", CSRC / "kernels" / "qrows.h", ROOT / "include" / "mi355x_kernels.h"]
+    hdrs = [CSRC / "kernels" / "common.h", CSRC / "kernels" / "decode_common.h", CSRC / "kernels" / "qrows.h", CSRC / "kernels" / "kv_cache.h", ROOT / "include" / "mi355x_kernels.h"]
     so = LIB / "libmi355x_kernels.so"
     if not _stale(so, [CSRC / "kernels" / s for s in KERNEL_SRCS] + hdrs) and not any((BUILD / "kernels").iterdir()):
         return so                                        # a library that travelled without its objects and is newer than its sources

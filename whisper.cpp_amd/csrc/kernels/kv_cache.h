@@ -1,0 +1,101 @@
+// Internal header of the paged K/V cache: what kv_cache.hip, attn_paged.hip and attn_packed.hip share.
+#pragma once
+#include "common.h"
+#include <atomic>
+
+// the calling thread's device is the context's for the length of a call, and the caller's again afterwards
+struct device_scope {
+    int prev = -1; bool changed = false;
+    explicit device_scope(const mi355x_ctx * ctx) {
+        if (hipGetDevice(&prev) == hipSuccess && prev != ctx->device) changed = hipSetDevice(ctx->device) == hipSuccess;
+    }
+    ~device_scope() { if (changed) (void) hipSetDevice(prev); }
+};
+
+// a cache as kernels see it
+struct kvc {
+    char * k, * v;
+    int64_t nb_key, nb_head, nb_page;
+    int * table, * len, * ref, * status, * work;
+    int n_pages, n_seq, max_pages, shift, mask, Hkv;
+};
+
+static inline int kv_refuse(const char * what) { mi355x_set_error("%s", what); return MI355X_E_UNSUPPORTED; }
+
+// argument checks of every call that takes a cache; fills `o`
+static inline int kv_view(const mi355x_kv_cache * c, kvc * o) {
+    if (!c) return kv_refuse("kv cache: NULL");
+    if (c->type != MI355X_TYPE_F16 && c->type != MI355X_TYPE_BF16) return kv_refuse("kv cache: type is neither F16 nor BF16");
+    if (c->head_dim != 64 && c->head_dim != 128) return kv_refuse("kv cache: head_dim is neither 64 nor 128");
+    if (c->n_head_kv < 1 || (int64_t) c->n_head_kv * c->head_dim > 32768) return kv_refuse("kv cache: n_head_kv");
+    if (c->page_size < 1 || c->page_size > 4096 || (c->page_size & (c->page_size - 1))) return kv_refuse("kv cache: page_size is not a power of two up to 4096");
+    if (c->n_pages < 1 || c->n_seq < 1 || c->n_seq > 262144 || c->max_pages < 1 || (int64_t) c->max_pages * c->page_size > INT32_MAX / 2) return kv_refuse("kv cache: n_pages, n_seq or max_pages");
+    if (!c->k || !c->v || !c->table || !c->len || !c->ref || !c->status || !c->work) return kv_refuse("kv cache: a NULL pointer");
+    if (((uintptr_t) c->k | (uintptr_t) c->v | (uintptr_t) c->nb_key | (uintptr_t) c->nb_head | (uintptr_t) c->nb_page) % 16) return kv_refuse("kv cache: pools and strides need 16-byte alignment");
+    if (((uintptr_t) c->table | (uintptr_t) c->len | (uintptr_t) c->ref | (uintptr_t) c->status | (uintptr_t) c->work) % 4) return kv_refuse("kv cache: misaligned tables");
+    const int64_t row = c->head_dim * 2;
+    if (c->nb_key < row || c->nb_head < row || c->nb_page < row) return kv_refuse("kv cache: strides smaller than a row");
+    o->k = (char *) c->k; o->v = (char *) c->v; o->nb_key = c->nb_key; o->nb_head = c->nb_head; o->nb_page = c->nb_page;
+    o->table = c->table; o->len = c->len; o->ref = c->ref; o->status = c->status; o->work = (int *) c->work;
+    o->n_pages = c->n_pages; o->n_seq = c->n_seq; o->max_pages = c->max_pages;
+    o->shift = __builtin_ctz((unsigned) c->page_size); o->mask = c->page_size - 1; o->Hkv = c->n_head_kv;
+    return 0;
+}
+
+// a tensor of rows of heads: [head_dim, heads, rows]
+static inline bool kv_rows_ok(const mi355x_tensor * t, int dim, int64_t heads) {
+    const int ts = t->type == MI355X_TYPE_F32 ? 4 : t->type == MI355X_TYPE_F16 || t->type == MI355X_TYPE_BF16 ? 2 : 0;
+    return ts && t->ne[0] == dim && t->ne[1] == heads && t->ne[2] >= 0 && t->ne[2] < INT32_MAX && t->ne[3] == 1 && t->nb[0] == ts &&
+           (t->data || t->ne[2] == 0) && ((uintptr_t) t->data | (uintptr_t) t->nb[1] | (uintptr_t) t->nb[2]) % 16 == 0;
+}
+
+// more than 64 KB of dynamic LDS has to be allowed once per kernel and device; `done`: a bit per device
+static inline int kv_allow_lds(mi355x_ctx * ctx, const void * f, uint32_t lds, std::atomic<uint64_t> & done) {
+    const uint64_t bit = 1ull << (ctx->device & 63);
+    if (lds <= 64 * 1024 || (done.load(std::memory_order_relaxed) & bit)) return 0;
+    const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024);
+    if (e != hipSuccess) { mi355x_set_error("dynamic LDS of %u bytes refused: %s", lds, hipGetErrorString(e)); return (int) e; }
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
+}
+
+#ifdef __HIPCC__
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef short  short4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+// the two 16-bit types: conversions (round to nearest even) and the matrix instructions on them
+struct f16_ops {
+    typedef half8_t vec8;
+    typedef half_t  elem;
+    static __device__ __forceinline__ floatx4  mfma16(vec8 a, vec8 b, floatx4 c)  { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ floatx16 mfma32(vec8 a, vec8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+struct bf16_ops {
+    typedef bf16x8_t vec8;
+    typedef __bf16   elem;
+    static __device__ __forceinline__ floatx4  mfma16(vec8 a, vec8 b, floatx4 c)  { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ floatx16 mfma32(vec8 a, vec8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+// eight consecutive elements of F32 / F16 / BF16 memory as floats, and back
+__device__ __forceinline__ void load8(const char * p, int type, float * f) {
+    if (type == MI355X_TYPE_F32) {
+        const float4 a = ((const float4 *) p)[0], b = ((const float4 *) p)[1];
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else if (type == MI355X_TYPE_F16) {
+        const half8_t a = *(const half8_t *) p;
+        #pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = (float) a[e];
+    } else {
+        const bf16x8_t a = *(const bf16x8_t *) p;
+        #pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = (float) a[e];
+    }
+}
+__device__ __forceinline__ void store4(char * p, int type, float a, float b, float c, float d) {
+    if (type == MI355X_TYPE_F32) *(float4 *) p = make_float4(a, b, c, d);
+    else if (type == MI355X_TYPE_F16) { half4_t h; h[0] = (half_t) a; h[1] = (half_t) b; h[2] = (half_t) c; h[3] = (half_t) d; *(half4_t *) p = h; }
+    else { typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4))); bf16x4_t h; h[0] = (__bf16) a; h[1] = (__bf16) b; h[2] = (__bf16) c; h[3] = (__bf16) d; *(bf16x4_t *) p = h; }
+}
+#endif

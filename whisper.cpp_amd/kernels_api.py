@@ -12,7 +12,7 @@ import numpy as np
 
 from . import KERNELS_SO
 
-F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, I32 = 0, 1, 2, 6, 8, 12, 26
+F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, I32, BF16 = 0, 1, 2, 6, 8, 12, 26, 30      # BF16: the paged K/V cache and its attentions only
 TYPE_NAMES = {"f32": F32, "f16": F16, "q4_0": Q4_0, "q5_0": Q5_0, "q8_0": Q8_0, "q4_k": Q4_K, "i32": I32}
 _BLOCK = {F32: (1, 4), F16: (1, 2), I32: (1, 4), Q4_0: (32, 18), Q5_0: (32, 22), Q8_0: (32, 34), Q4_K: (256, 144)}
 
@@ -25,6 +25,8 @@ SYMBOLS = [
     "mi355x_flash_attn_ext", "mi355x_flash_attn_ext_exact", "mi355x_flash_attn_partial", "mi355x_flash_attn_combine", "mi355x_norm", "mi355x_binary", "mi355x_scale", "mi355x_gelu", "mi355x_cpy",
     "mi355x_last_launch_mirrored", "mi355x_act_planes_bytes", "mi355x_act_prepare", "mi355x_act_scratch", "mi355x_flash_attn_partial_multi", "mi355x_flash_attn_planes", "mi355x_decode_head_multi",
     "mi355x_argmax_top2", "mi355x_act_rows_bytes", "mi355x_gemm_q8act", "mi355x_gemm_q8act_prep", "mi355x_flash_attn_ext_prep_rows", "mi355x_unary", "mi355x_pad_reflect_1d", "mi355x_get_rows", "mi355x_get_rows_add", "mi355x_im2col_1d", "mi355x_soft_max", "mi355x_rope", "mi355x_concat", "mi355x_memset", "mi355x_checksum", "mi355x_log_mel", "mi355x_log_mel_n_len", "mi355x_debug_read_stamps", "mi355x_wake", "mi355x_test_option",
+    "mi355x_kv_work_bytes", "mi355x_kv_reset", "mi355x_kv_append", "mi355x_kv_truncate", "mi355x_kv_fork", "mi355x_kv_compact",
+    "mi355x_attn_paged_work_bytes", "mi355x_attn_paged", "mi355x_attn_packed",
 ]
 
 
@@ -89,6 +91,25 @@ class RopeParams(C.Structure):
     _fields_ = [("n_dims", C.c_int32), ("mode", C.c_int32), ("n_ctx_orig", C.c_int32), ("freq_base", C.c_float),
                 ("freq_scale", C.c_float), ("ext_factor", C.c_float), ("attn_factor", C.c_float), ("beta_fast", C.c_float),
                 ("beta_slow", C.c_float), ("sections", C.c_int32 * 4)]
+
+
+class KvCache(C.Structure):           # mi355x_kv_cache
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int32), ("head_dim", C.c_int32), ("n_head_kv", C.c_int32), ("page_size", C.c_int32),
+                ("n_pages", C.c_int32), ("n_seq", C.c_int32), ("max_pages", C.c_int32), ("reserved", C.c_int32), ("nb_key", C.c_int64), ("nb_head", C.c_int64),
+                ("nb_page", C.c_int64), ("table", C.c_void_p), ("len", C.c_void_p), ("ref", C.c_void_p), ("status", C.c_void_p), ("work", C.c_void_p)]
+
+
+KV_BAD_ARG, KV_ROW_FULL, KV_OUT_OF_PAGES = 1, 2, 4      # enum mi355x_kv_status
+
+
+class AttnPagedDesc(C.Structure):
+    _fields_ = [("q", Tensor), ("dst", Tensor), ("seq", C.c_void_p), ("scale", C.c_float), ("window", C.c_int32), ("max_len", C.c_int32), ("reserved", C.c_int32),
+                ("work", C.c_void_p), ("work_bytes", C.c_size_t)]
+
+
+class AttnPackedDesc(C.Structure):
+    _fields_ = [("q", Tensor), ("k", Tensor), ("v", Tensor), ("dst", Tensor), ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("cache", C.POINTER(KvCache)),
+                ("seq", C.c_void_p), ("n", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32), ("max_q", C.c_int32), ("scale", C.c_float), ("reserved", C.c_int32)]
 
 
 class ProfRow(C.Structure):
@@ -160,6 +181,18 @@ def lib() -> C.CDLL:
         L.mi355x_checksum.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
         L.mi355x_log_mel_n_len.argtypes = [C.c_int]
         L.mi355x_log_mel.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_int]
+        CP = C.POINTER(KvCache)
+        L.mi355x_kv_work_bytes.restype = C.c_size_t
+        L.mi355x_kv_work_bytes.argtypes = [C.c_int, C.c_int]
+        L.mi355x_kv_reset.argtypes = [C.c_void_p, CP]
+        L.mi355x_kv_append.argtypes = [C.c_void_p, CP, C.c_int, C.c_void_p, C.c_void_p, TP, TP]
+        L.mi355x_kv_truncate.argtypes = [C.c_void_p, CP, C.c_int, C.c_void_p, C.c_void_p]
+        L.mi355x_kv_fork.argtypes = [C.c_void_p, CP, C.c_int, C.c_void_p, C.c_void_p]
+        L.mi355x_kv_compact.argtypes = [C.c_void_p, CP, CP]
+        L.mi355x_attn_paged_work_bytes.restype = C.c_size_t
+        L.mi355x_attn_paged_work_bytes.argtypes = [CP, C.c_int, C.c_int, C.c_int]
+        L.mi355x_attn_paged.argtypes = [C.c_void_p, CP, C.POINTER(AttnPagedDesc)]
+        L.mi355x_attn_packed.argtypes = [C.c_void_p, C.POINTER(AttnPackedDesc)]
         L.mi355x_memset.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_size_t]
         L.mi355x_debug_read_stamps.argtypes = [C.c_void_p, C.POINTER(C.c_uint64)]
         _lib = L
@@ -205,6 +238,66 @@ def repack_from_planar(t: int, planar: np.ndarray, nelements: int) -> np.ndarray
     return dst
 
 
+# ---- the paged K/V cache and its attentions, on device arrays (torch tensors or anything with data_ptr / shape / stride / dtype) ----
+_DTYPE = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+
+
+def _rows(t) -> Tensor:
+    """[rows, heads, dim] as the C side's [dim, heads, rows]"""
+    if t.dim() != 3 or str(t.dtype) not in _DTYPE:
+        raise ValueError(f"expected [rows, heads, dim] of float32, float16 or bfloat16, got {list(t.shape)} {t.dtype}")
+    b = t.element_size()
+    return tensor(t.data_ptr(), _DTYPE[str(t.dtype)], [t.shape[2], t.shape[1], t.shape[0]], [t.stride(2) * b, t.stride(1) * b, t.stride(0) * b])
+
+
+def _ints(t, n: int, what: str):
+    """the address of at least n contiguous 32-bit integers"""
+    if t is None:
+        return None
+    if str(t.dtype) != "torch.int32" or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{what}: {n} contiguous int32 values wanted, got {list(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def kv_work_bytes(n_seq: int, n_pages: int) -> int:
+    return lib().mi355x_kv_work_bytes(n_seq, n_pages)
+
+
+def kv_cache(k, v, table, length, ref, status, work) -> KvCache:
+    """Describe a paged cache: pools k, v [page, head, key, dim] (any order of heads and keys in memory), table [sequence, page], length [sequence],
+    ref [page], status [1] int32, work: kv_work_bytes() bytes.  The arrays have to outlive the description."""
+    if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.dim() != 4 or str(k.dtype) not in _DTYPE or k.stride(3) != 1:
+        raise ValueError("k and v: [page, head, key, dim] of one shape, type and layout, dims contiguous")
+    if table.dim() != 2:
+        raise ValueError("table: [sequence, page]")
+    b, need = k.element_size(), kv_work_bytes(table.shape[0], k.shape[0])
+    if work.numel() * work.element_size() < need or not work.is_contiguous():
+        raise ValueError(f"work: {need} bytes wanted")
+    c = KvCache()
+    c.k, c.v, c.type, c.head_dim, c.n_head_kv, c.page_size = k.data_ptr(), v.data_ptr(), _DTYPE[str(k.dtype)], k.shape[3], k.shape[1], k.shape[2]
+    c.n_pages, c.n_seq, c.max_pages = k.shape[0], table.shape[0], table.shape[1]
+    c.nb_key, c.nb_head, c.nb_page = k.stride(2) * b, k.stride(1) * b, k.stride(0) * b
+    c.table, c.len, c.ref = _ints(table, 0, "table"), _ints(length, c.n_seq, "length"), _ints(ref, c.n_pages, "ref")
+    c.status, c.work = _ints(status, 1, "status"), work.data_ptr()
+    return c
+
+
+def attn_paged_work_bytes(cache: KvCache, n: int, n_head: int, max_len: int = 0) -> int:
+    return lib().mi355x_attn_paged_work_bytes(C.byref(cache), n, n_head, max_len)
+
+
+class Call:
+    """A call of the C ABI with its arguments made once: a decode loop repeats it with new contents of the same arrays."""
+
+    def __init__(self, ctx, name: str, *args, keep=()):
+        self.ctx, self.name, self.fn, self.args, self.keep = ctx, name, getattr(lib(), name), (ctx.h, *args), (args, keep)
+
+    def __call__(self):
+        rc = self.fn(*self.args)
+        if rc:
+            self.ctx.check(rc, self.name)
+
+
 class Ctx:
     """One kernel context (HIP stream + scratch).  Raises if no gfx950 device is usable."""
 
@@ -226,6 +319,41 @@ class Ctx:
         if self.h:
             lib().mi355x_ctx_destroy(self.h)
             self.h = None
+
+    # ---- the paged cache: each returns a Call (arrays as in kv_cache(); lists int32 on the device) ----
+    def kv_reset_call(self, cache: KvCache) -> Call:
+        return Call(self, "mi355x_kv_reset", C.byref(cache), keep=cache)
+
+    def kv_append_call(self, cache: KvCache, seq, cu, k, v) -> Call:
+        n, tk, tv = seq.numel(), _rows(k), _rows(v)
+        return Call(self, "mi355x_kv_append", C.byref(cache), n, _ints(seq, n, "seq"), _ints(cu, n + 1, "cu"), C.byref(tk), C.byref(tv), keep=(cache, seq, cu, k, v))
+
+    def kv_truncate_call(self, cache: KvCache, seq, keep) -> Call:
+        n = seq.numel()
+        return Call(self, "mi355x_kv_truncate", C.byref(cache), n, _ints(seq, n, "seq"), _ints(keep, n, "keep"), keep=(cache, seq, keep))
+
+    def kv_fork_call(self, cache: KvCache, src, dst) -> Call:
+        n = src.numel()
+        return Call(self, "mi355x_kv_fork", C.byref(cache), n, _ints(src, n, "src"), _ints(dst, n, "dst"), keep=(cache, src, dst))
+
+    def kv_compact_call(self, cache: KvCache, to: KvCache) -> Call:
+        return Call(self, "mi355x_kv_compact", C.byref(cache), C.byref(to), keep=(cache, to))
+
+    def attn_paged_call(self, cache: KvCache, q, out, seq=None, scale: float = 1.0, window: int = 0, max_len: int = 0, work=None) -> Call:
+        d = AttnPagedDesc()
+        d.q, d.dst, d.seq, d.scale, d.window, d.max_len = _rows(q), _rows(out), _ints(seq, q.shape[0], "seq"), scale, window, max_len
+        d.work, d.work_bytes = (work.data_ptr() or None, work.numel() * work.element_size()) if work is not None else (None, 0)
+        return Call(self, "mi355x_attn_paged", C.byref(cache), C.byref(d), keep=(cache, d, q, out, seq, work))
+
+    def attn_packed_call(self, q, out, cu_q, k=None, v=None, cu_k=None, cache=None, seq=None, scale: float = 1.0, causal: bool = True, window: int = 0, max_q: int = 0) -> Call:
+        d, n = AttnPackedDesc(), cu_q.numel() - 1
+        d.q, d.dst, d.cu_q, d.n = _rows(q), _rows(out), _ints(cu_q, 1, "cu_q"), n
+        if cache is not None:
+            d.cache, d.seq = C.pointer(cache), _ints(seq, n, "seq")
+        else:
+            d.k, d.v, d.cu_k = _rows(k), _rows(v), _ints(cu_k, n + 1, "cu_k")
+        d.scale, d.causal, d.window, d.max_q = scale, causal, window, max_q
+        return Call(self, "mi355x_attn_packed", C.byref(d), keep=(cache, d, q, out, cu_q, k, v, cu_k, seq))
 
     def prof(self, on: bool):
         lib().mi355x_prof_enable(self.h, 1 if on else 0)
