@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     constexpr int KK = D / 32;                           // 32-dim pieces of a key
     constexpr int NV = D / 16;                           // V loads of a tile; 16-dim blocks of the result
     constexpr int RPL = 512 / D;                         // V rows per load
-    extern __shared__ char lds[];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, nl = lane & 15, g4 = lane >> 4, waves = blockDim.x >> 6;
     const int unit = blockIdx.x, grp = unit % a.groups, hk = unit / a.groups % a.c.Hkv, i = unit / a.groups / a.c.Hkv, share = blockIdx.y;
     const paged_span sp = span_of(a, i);
