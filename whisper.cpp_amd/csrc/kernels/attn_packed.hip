@@ -14,68 +14,27 @@
 // out on the way into LDS and counted over the keys that a row sees, so that a row never meets what it does not see.
 #include "kv_cache.h"
 
-#define KT 64                          // keys of a tile
 
-struct PackedArgs {
-    kvc c;                             // PAGED: the cache.  Otherwise k, v and their strides in nb_key (rows) and nb_head
-    const char * q; int64_t q_nb1, q_nb2;
-    char * o; int64_t o_nb1, o_nb2;
-    const int * cu_q, * cu_k, * seq;
-    float c2; int flip;                // |scale| * log2(e), at least 1e-37; whether the scale is negative (the queries change sign)
-    int n, rows_q, rows_k, q_type, o_type, causal, window;
-    int G, Hkv, qt;                    // query heads per K/V head; queries of a workgroup
-};
+// what a 16-byte piece's number in its row is changed by (exclusive-or): the rows that an instruction reads together lie in different banks
+template <int D> __device__ __forceinline__ int k_swap(int key) { return D == 128 ? key & 15 : key >> 1 & 7; }
+template <int D> __device__ __forceinline__ int v_swap(int key) { return D == 128 ? (key & 3) << 2 : (key >> 1 & 1) << 2; }
+#define LDS __attribute__((address_space(3)))
+__device__ __forceinline__ uint32_t lds_at(char * p) { return (uint32_t) (size_t) (LDS char *) p; }
 
-// slot -> (sequence, tile of its rows): sequence i has the slots cu[i]/qt + i .. cu[i+1]/qt + i, at least as many as its tiles, found by bisection
-struct packed_job { int i, r0, nq, L, tile; };
-__device__ __forceinline__ bool packed_find(const PackedArgs & a, int slot, packed_job & j) {
-    int lo = 0, hi = a.n;
-    while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (a.cu_q[m] / a.qt + m <= slot) lo = m; else hi = m; }
-    j.i = lo;
-    j.r0 = a.cu_q[lo]; const int r1 = a.cu_q[lo + 1];
-    if (j.r0 < 0 || r1 > a.rows_q || r1 <= j.r0) return false;
-    j.nq = r1 - j.r0;
-    const int tiles = (j.nq + a.qt - 1) / a.qt, t = slot - (j.r0 / a.qt + lo);
-    if (t < 0 || t >= tiles) return false;
-    j.tile = tiles - 1 - t;                                          // the rows with most keys first
-    return true;
-}
-
-template <typename O, int D> __device__ __forceinline__ int k_piece(int key, int piece) { return D == 128 ? piece ^ (key & 15) : piece ^ ((key >> 1) & 7); }
-template <int D> __device__ __forceinline__ int v_slot(int key, int piece) { return D == 128 ? piece ^ ((key & 3) << 2) : piece ^ (((key >> 1) & 1) << 2); }
-
-// bit 15 of each half: whether it is an infinity or a NaN
-template <typename O> __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
-    return ((w & 0x7FFF7FFFu) + (__is_same(O, f16_ops) ? 0x04000400u : 0x00800080u)) & 0x80008000u;
-}
-template <typename O> __device__ __forceinline__ uint32_t not_finite8(u32x4_t w) { return not_finite2<O>(w[0]) | not_finite2<O>(w[1]) | not_finite2<O>(w[2]) | not_finite2<O>(w[3]); }
-
-// infinities and NaNs out of eight values: zeros in their places, and what they were as numbers of the type: 1 (inf), 128 (-inf), 16384 (NaN)
-template <typename O> __device__ __forceinline__ void take_apart(u32x4_t & v, u32x4_t & kind) {
-    constexpr bool F = __is_same(O, f16_ops);
-    #pragma unroll
-    for (int w = 0; w < 4; w++)
-        #pragma unroll
-        for (int h = 0; h < 32; h += 16) {
-            const uint32_t x = v[w] >> h & 0xFFFF, top = F ? 0x7C00 : 0x7F80;
-            if ((x & top) != top) continue;
-            kind[w] |= ((x & 0x7FFF) != top ? (F ? 0x7400u : 0x4680u) : x & 0x8000 ? (F ? 0x5800u : 0x4300u) : (F ? 0x3C00u : 0x3F80u)) << h;
-            v[w] &= ~(0xFFFFu << h);
-        }
-}
-
-#define SLOTS 3                        // K tiles t .. t+2, V tiles t-1 .. t+1 are in use at a time
-
-template <typename O, int D, bool PAGED>
-__global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
+template <typename O, int D, bool PAGED, int NW, int KG>
+__global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) {
     typedef typename O::vec8 vec8;
     typedef typename O::elem elem;
     constexpr int KK = D / 16, NI = D / 32;
     constexpr int PCS = D / 8;                                        // 16-byte pieces of a row
-    constexpr int NL = KT * PCS / 512, RPL = 512 / PCS;               // pieces per thread and tile, K and V each; keys that lie between them
+    constexpr int KT = NW == 8 || KG == 2 ? 64 : 32;                             // keys of a tile
+    constexpr int KA = NW == 8 ? 2 : 1, VA = KA - 1;                  // tiles that K and V are in LDS ahead of the step that they are written in
+    constexpr int SLOTS = NW == 8 ? 3 : 1;                            // in use at a time: K tiles t .. t+2, V tiles t-1 .. t+1 (one of each where all waves are in step)
+    constexpr int NL = KT * PCS / (64 * NW), RPL = 64 * NW / PCS;               // pieces per thread and tile, K and V each; keys that lie between them
     constexpr int TILE_B = KT * D * 2;
-    extern __shared__ __attribute__((aligned(16))) char lds[];                                     // SLOTS K tiles, SLOTS V tiles, SLOTS tiles of what was taken out of V
-    __shared__ int odd[SLOTS];                                        // t + 1: something was taken out of V tile t
+    constexpr int NB = KT / 32 / KG, NC = 2 * NB;                     // 32-key blocks of S and 16-key chunks of P that a wave has of a tile
+    extern __shared__ __attribute__((aligned(1024))) char lds[];      // SLOTS K tiles, SLOTS V tiles, SLOTS tiles of what was taken out of V, odd[SLOTS]
+    int * odd = (int *) (lds + 3 * SLOTS * TILE_B);                   // t + 1: something was taken out of V tile t
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, hf = lane >> 5;
     const int hk = blockIdx.x % a.Hkv, slot = blockIdx.x / a.Hkv;
     packed_job job;
@@ -94,21 +53,22 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
         k0 = a.cu_k[job.i]; const int k1 = a.cu_k[job.i + 1];
         if (k0 >= 0 && k1 <= a.rows_k && k1 > k0) L = k1 - k0;
     }
-    // this lane's row
-    const int q_base = job.tile * a.qt, nrow = min(a.qt, job.nq - q_base) * a.G, r = wave * 32 + (lane & 31);
+    // this lane's row; which half of each tile's keys this wave takes (KG 2)
+    const int rw = wave % (NW / KG), k_off = wave / (NW / KG) * 32;
+    const int q_base = job.tile * a.qt, nrow = min(a.qt, job.nq - q_base) * a.G, r = rw * 32 + (lane & 31);
     const int rc = min(r, nrow - 1), qi = q_base + rc / a.G, g = rc - rc / a.G * a.G;
     const int off = L - job.nq;                                       // row qi's own key is off + qi
     const int last = a.causal ? min(off + qi, L - 1) : L - 1;         // the last key it sees (-1: none)
     const int first = a.window > 0 ? max(off + qi - a.window + 1, 0) : 0;
     // the same for the wave's first and last row and for the workgroup's: uniform
-    const int wr0 = min(wave * 32, nrow - 1), wr1 = min(wave * 32 + 31, nrow - 1), wq0 = q_base + wr0 / a.G, wq1 = q_base + wr1 / a.G, bq1 = q_base + (nrow - 1) / a.G;
+    const int wr0 = min(rw * 32, nrow - 1), wr1 = min(rw * 32 + 31, nrow - 1), wq0 = q_base + wr0 / a.G, wq1 = q_base + wr1 / a.G, bq1 = q_base + (nrow - 1) / a.G;
     const int w_last_min = a.causal ? min(off + wq0, L - 1) : L - 1, w_last = a.causal ? min(off + wq1, L - 1) : L - 1;
     const int w_first = a.window > 0 ? max(off + wq0 - a.window + 1, 0) : 0, w_first_max = a.window > 0 ? max(off + wq1 - a.window + 1, 0) : 0;
     const int b_last_min = a.causal ? min(off + q_base, L - 1) : L - 1, b_last = a.causal ? min(off + bq1, L - 1) : L - 1;
     const int b_first = a.window > 0 ? max(off + q_base - a.window + 1, 0) : 0, b_first_max = a.window > 0 ? max(off + bq1 - a.window + 1, 0) : 0;
     const int T0 = b_first / KT, T = b_last >= b_first && L > 0 ? b_last / KT + 1 - T0 : 0;          // tiles T0 .. T0 + T - 1
     // tiles that this wave's rows see nothing of are passed over; the rest of its tiles are t_lo .. t_hi - 1
-    const int t_lo = max(w_first / KT - T0, 0), t_hi = wave * 32 < nrow && w_last >= w_first ? min(w_last / KT + 1 - T0, T) : 0;
+    const int t_lo = max(w_first / KT - T0, 0), t_hi = rw * 32 < nrow && w_last >= w_first ? min(w_last / KT + 1 - T0, T) : 0;
 
     vec8 qf[KK];
     {
@@ -121,8 +81,8 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
             for (int e = 0; e < 8; e++) qf[kk][e] = (elem) (a.flip ? -f[e] : f[e]);
         }
     }
-    floatx16 o[NI], s[2];
-    vec8 pf[4];
+    floatx16 o[NI], s[NB];
+    vec8 pf[NC];
     #pragma unroll
     for (int i = 0; i < NI; i++)
         #pragma unroll
@@ -156,17 +116,17 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
         #pragma unroll
         for (int e = 0; e < NL; e++) vr[e] = *(const u32x4_t *) (vb + place(t, e, pg));
     };
+    const int k_put = skey * (D * 2) + (spc ^ k_swap<D>(skey)) * 16, v_put = skey * (D * 2) + (spc ^ v_swap<D>(skey)) * 16;     // (the same for keys RPL apart)
     auto put_k = [&](int t) {
-        char * kl = lds + t % SLOTS * TILE_B;
         #pragma unroll
-        for (int e = 0; e < NL; e++) *(u32x4_t *) (kl + (skey + e * RPL) * (D * 2) + k_piece<O, D>(skey + e * RPL, spc) * 16) = kr[e];
+        for (int e = 0; e < NL; e++) *(u32x4_t *) (lds + t % SLOTS * TILE_B + k_put + e * RPL * (D * 2)) = kr[e];
     };
     auto put_v = [&](int t) {
-        char * vl = lds + (SLOTS + t % SLOTS) * TILE_B;
+        char * vl = lds + (SLOTS + t % SLOTS) * TILE_B + v_put;
         const bool edge = (T0 + t) * KT + KT - 1 > b_last_min || (T0 + t) * KT < b_first_max;         // masked in part for some row
         #pragma unroll
         for (int e = 0; e < NL; e++) {
-            const int at = (skey + e * RPL) * (D * 2) + v_slot<D>(skey + e * RPL, spc) * 16;
+            const int at = e * RPL * (D * 2);
             if (edge) {
                 u32x4_t kind = { 0, 0, 0, 0 };
                 if (not_finite8<O>(vr[e])) { take_apart<O>(vr[e], kind); odd[t % SLOTS] = t + 1; }    // every writer writes the same; what an older tile left does not match
@@ -175,69 +135,70 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
             *(u32x4_t *) (vl + at) = vr[e];
         }
     };
+    // a lane's places in a K tile (key lane & 31, piece 2 kk + hf: exclusive-or with kk << 5) and in a V tile (4 hf + (lane & 15) / 4, half a piece of dims
+    // 32 i + 16 (lane / 16 & 1) ..: exclusive-or with i << 6)
+    const int li = lane & 15, key0 = 4 * hf + (li >> 2);
+    const uint32_t k_lane = (lane & 31) * (D * 2) + (hf ^ k_swap<D>(lane & 31)) * 16;
+    const uint32_t v_lane = key0 * (D * 2) + ((2 * ((lane >> 4) & 1) + ((li >> 1) & 1)) ^ v_swap<D>(key0)) * 16 + (li & 1) * 8;
     auto part = [&](int t) { return (T0 + t) * KT + KT - 1 > w_last_min || (T0 + t) * KT < w_first_max; };
 
-    // S^T = K.Q^T: element e of block b is key 32 b + (e & 3) + 8 (e >> 2) + 4 hf of the tile
+    // S^T = K.Q^T: element e of block b is key k_off + 32 b + (e & 3) + 8 (e >> 2) + 4 hf of the tile
     auto qk = [&](int t) {
-        const char * kl = lds + t % SLOTS * TILE_B;
+        const uint32_t kl = lds_at(lds) + t % SLOTS * TILE_B + k_off * (D * 2) + k_lane;
         #pragma unroll
-        for (int b = 0; b < 2; b++)
+        for (int b = 0; b < NB; b++)
             #pragma unroll
             for (int e = 0; e < 16; e++) s[b][e] = 0.0f;
-        vec8 kf[2][2];                                                // the next products' operands are read while these run
+        vec8 kf[4][NB];                                               // the next products' operands are read while these run
         auto get = [&](int kk) {
             #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const int key = b * 32 + (lane & 31);
-                kf[kk & 1][b] = *(const vec8 *) (kl + key * (D * 2) + k_piece<O, D>(key, kk * 2 + hf) * 16);
+            for (int b = 0; b < NB; b++) {
+                kf[kk & 3][b] = *(const LDS vec8 *) (size_t) ((kl ^ kk << 5) + b * 32 * (D * 2));
             }
         };
-        get(0);
+        get(0); get(1); get(2);
         #pragma unroll
         for (int kk = 0; kk < KK; kk++) {
-            if (kk + 1 < KK) get(kk + 1);
+            if (kk + 3 < KK) get(kk + 3);
             #pragma unroll
-            for (int b = 0; b < 2; b++) s[b] = O::mfma32(kf[kk & 1][b], qf[kk], s[b]);
+            for (int b = 0; b < NB; b++) s[b] = O::mfma32(kf[kk & 3][b], qf[kk], s[b]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // V^T's operand for keys 16 c .. +15 (this lane's 16-lane group: 16 c + 4 hf + {0..3} and + 8), dims 32 i .. +31
-    auto v_frag = [&](const char * vl, int c, int i) {
-        const int li = lane & 15;
+    // V^T's operand for keys k_off + 16 c .. +15 (this lane's 16-lane group: 4 hf + {0..3} and + 8 of them), dims 32 i .. +31
+    auto v_frag = [&](uint32_t vl, int c, int i) {
         vec8 vf;
         #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const int key = 16 * c + 4 * hf + (li >> 2) + 8 * b;
-            const char * at = vl + key * (D * 2) + v_slot<D>(key, 4 * i + 2 * ((lane >> 4) & 1) + ((li >> 1) & 1)) * 16 + (li & 1) * 8;
-            const short4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *) at);
+            const short4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS short4_t *) (size_t) ((vl ^ i << 6) + (16 * c + 8 * b) * (D * 2)));
             __builtin_memcpy((char *) &vf + 8 * b, &x, 8);
         }
         return vf;
     };
     // O^T += V^T.P^T
     auto pv = [&](int t) {
-        const char * vl = lds + (SLOTS + t % SLOTS) * TILE_B;
+        const uint32_t vl = lds_at(lds) + (SLOTS + t % SLOTS) * TILE_B + k_off * (D * 2) + v_lane;
         vec8 vf[2][NI];
         #pragma unroll
         for (int i = 0; i < NI; i++) vf[0][i] = v_frag(vl, 0, i);
         #pragma unroll
-        for (int c = 0; c < 4; c++) {
+        for (int c = 0; c < NC; c++) {
             #pragma unroll
-            for (int i = 0; i < NI; i++) if (c + 1 < 4) vf[(c + 1) & 1][i] = v_frag(vl, c + 1, i);
+            for (int i = 0; i < NI; i++) if (c + 1 < NC) vf[(c + 1) & 1][i] = v_frag(vl, c + 1, i);
             #pragma unroll
             for (int i = 0; i < NI; i++) o[i] = O::mfma32(vf[c & 1][i], pf[c], o[i]);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (__builtin_amdgcn_readfirstlane(odd[t % SLOTS]) != t + 1) return;
         // what was taken out of this tile, for the rows that see it: over the visible keys, how many of each kind
-        const int hi = last - (T0 + t) * KT - 4 * hf, lo = first - (T0 + t) * KT - 4 * hf;
+        const int hi = last - (T0 + t) * KT - k_off - 4 * hf, lo = first - (T0 + t) * KT - k_off - 4 * hf;
         #pragma unroll
         for (int i = 0; i < NI; i++) {
             floatx16 cnt;
             #pragma unroll
             for (int e = 0; e < 16; e++) cnt[e] = 0.0f;
             #pragma unroll
-            for (int c = 0; c < 4; c++) {
+            for (int c = 0; c < NC; c++) {
                 vec8 seen;
                 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -249,8 +210,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
             }
             #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const int n = (int) cnt[e];                           // NaNs x 16384 + (-inf)s x 128 + (+inf)s, at most 64 of each
-                o[i][e] += ((n & 127) ? INFINITY : 0.0f) + ((n & 0x3F80) ? -INFINITY : 0.0f) + (n >= 16384 ? NAN : 0.0f);
+                o[i][e] += put_back(cnt[e]);
             }
         }
     };
@@ -258,9 +218,9 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
     // hardly ever rescaled; F16 weights are held times 2^7 (2^15 at most), so that small ones do not fall below its range.  Both cancel against the sum.
     auto softmax = [&](int t) {
         if (part(t)) {
-            const int hi = last - (T0 + t) * KT - 4 * hf, lo = first - (T0 + t) * KT - 4 * hf;
+            const int hi = last - (T0 + t) * KT - k_off - 4 * hf, lo = first - (T0 + t) * KT - k_off - 4 * hf;
             #pragma unroll
-            for (int b = 0; b < 2; b++)
+            for (int b = 0; b < NB; b++)
                 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int k = 32 * b + (e & 3) + 8 * (e >> 2);
@@ -269,7 +229,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
         }
         float top = fmaxf(s[0][0], s[0][1]);
         #pragma unroll
-        for (int e = 2; e < 32; e += 2) top = fmaxf(fmaxf(top, s[e >> 4][e & 15]), s[(e + 1) >> 4][(e + 1) & 15]);
+        for (int e = 2; e < 16 * NB; e += 2) top = fmaxf(fmaxf(top, s[e >> 4][e & 15]), s[(e + 1) >> 4][(e + 1) & 15]);
         top = fmaxf(top, lane_xor32(top));
         if (__any((top - m) * a.c2 > 8.0f)) {
             const float mn = fmaxf(m, top), alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * a.c2);
@@ -282,7 +242,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
         const float mc = (m == -INFINITY ? 0.0f : m * a.c2) - (__is_same(O, f16_ops) ? 7.0f : 0.0f);
         float sum = 0.0f;
         #pragma unroll
-        for (int b = 0; b < 2; b++)
+        for (int b = 0; b < NB; b++)
             #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], a.c2, -mc));
@@ -293,40 +253,48 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
     };
 
     if (T > 0) {
-        // Two groups of four waves, one of each on every SIMD, half a step apart: while one runs the matrix products of a step (PV of the tile before, QK
-        // of this one), the other runs the softmax and brings tiles in.  A barrier ends each half step.
-        const bool second = wave >= 4;
+        // Eight waves: two groups of four, one wave of each on every SIMD, half a step apart: while one runs the matrix products of a step (PV of the tile
+        // before, QK of this one), the other runs the softmax and brings tiles in.  A barrier ends each half step.  Four waves: all in step, another
+        // workgroup of the CU fills the gaps.
+        const bool second = NW == 8 && wave >= 4;
         if (tid < SLOTS) odd[tid] = 0;
         page_of(0, pg_k);
         page_of(min(1, T - 1), pg_n);
         fetch_k(0, pg_k);
-        fetch_v(0, pg_k);
+        if (VA == 1) fetch_v(0, pg_k);
         put_k(0);
-        fetch_k(min(1, T - 1), pg_n);
-        __syncthreads();                                              // odd[] cleared
-        put_v(0);
-        put_k(1);
-        #pragma unroll
-        for (int e = 0; e < NL; e++) pg_v[e] = pg_n[e];               // V tile 1, K tile 2 next
-        page_of(min(2, T - 1), pg_k);
-        fetch_v(min(1, T - 1), pg_v);
-        fetch_k(min(2, T - 1), pg_k);
-        page_of(min(3, T - 1), pg_n);
+        if (KA == 2) {
+            fetch_k(min(1, T - 1), pg_n);
+            __syncthreads();                                          // odd[] cleared
+            put_v(0);
+            put_k(1);
+            #pragma unroll
+            for (int e = 0; e < NL; e++) { pg_v[e] = pg_n[e]; }
+            page_of(min(2, T - 1), pg_k);
+        } else {
+            #pragma unroll
+            for (int e = 0; e < NL; e++) { pg_v[e] = pg_k[e]; pg_k[e] = pg_n[e]; }
+        }
+        fetch_v(min(VA, T - 1), pg_v);                                // V tile VA, K tile KA next
+        fetch_k(min(KA, T - 1), pg_k);
+        page_of(min(KA + 1, T - 1), pg_n);
         __syncthreads();
         if (second) __syncthreads();
         for (int t = 0; t < T; t++) {
+            if (NW == 8) __builtin_amdgcn_s_setprio(1);
             if (t > t_lo && t <= t_hi) pv(t - 1);
             if (t >= t_lo && t < t_hi) qk(t);
+            if (NW == 8) __builtin_amdgcn_s_setprio(0);
             __syncthreads();
-            if (t + 2 < T) put_k(t + 2);
-            if (t + 1 < T) put_v(t + 1);
-            if (t + 3 < T) {
+            if (t + KA < T) put_k(t + KA);
+            if (t + VA < T) put_v(t + VA);
+            if (t + KA + 1 < T) {
                 #pragma unroll
                 for (int e = 0; e < NL; e++) { pg_v[e] = pg_k[e]; pg_k[e] = pg_n[e]; }
-                fetch_k(t + 3, pg_k);
-                page_of(min(t + 4, T - 1), pg_n);
-                fetch_v(t + 2, pg_v);
-            } else if (t + 2 < T) fetch_v(t + 2, pg_k);
+                fetch_k(t + KA + 1, pg_k);
+                page_of(min(t + KA + 2, T - 1), pg_n);
+                fetch_v(t + VA + 1, pg_v);
+            } else if (t + VA + 1 < T) fetch_v(t + VA + 1, pg_k);
             if (t >= t_lo && t < t_hi) softmax(t);
             if (!second || t + 1 < T) __syncthreads();
         }
@@ -334,6 +302,27 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
     }
     if (PAGED && __any(bad) && lane == 0) atomicOr((unsigned *) a.c.status, MI355X_KV_BAD_ARG);
     l += lane_xor32(l);
+    if (KG == 2) {                                                    // the second half of the keys joins the first, over the dead tiles: [m, l, o ..][wave, lane]
+        constexpr int RS = 32 * NW;                                   // records are laid lane by lane
+        float * rec = (float *) lds + (wave % (NW / 2)) * 64 + lane;
+        __syncthreads();
+        if (wave >= NW / 2) {
+            rec[0] = m; rec[RS] = l;
+            #pragma unroll
+            for (int i = 0; i < NI; i++)
+                #pragma unroll
+                for (int e = 0; e < 16; e++) rec[(2 + 16 * i + e) * RS] = o[i][e];
+        }
+        __syncthreads();
+        if (wave >= NW / 2) return;
+        const float mo = rec[0], mn = fmaxf(m, mo);
+        const float f0 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * a.c2), f1 = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mo - mn) * a.c2);
+        l = l * f0 + rec[RS] * f1;
+        #pragma unroll
+        for (int i = 0; i < NI; i++)
+            #pragma unroll
+            for (int e = 0; e < 16; e++) o[i][e] = o[i][e] * f0 + rec[(2 + 16 * i + e) * RS] * f1;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (r < nrow) {
         char * op = a.o + (int64_t) (job.r0 + qi) * a.o_nb2 + (int64_t) (hk * a.G + g) * a.o_nb1;
@@ -345,13 +334,41 @@ __global__ void __launch_bounds__(512, 2) k_attn_packed(const PackedArgs a) {
     }
 }
 
-template <typename O, int D, bool PAGED>
-static int launch_packed(mi355x_ctx * ctx, const PackedArgs & a, int64_t blocks) {
+template <typename O, int D, bool PAGED, int NW, int KG>
+static int launch_packed_as(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv) {
     static std::atomic<uint64_t> allowed{0};
-    const uint32_t lds = 3 * SLOTS * KT * D * 2;
-    const int rl = kv_allow_lds(ctx, (const void *) k_attn_packed<O, D, PAGED>, lds + 1024, allowed);
+    a.qt = 32 * NW / KG / a.G;
+    const int64_t blocks = ((int64_t) a.rows_q / a.qt + a.n) * Hkv;
+    if (blocks > INT32_MAX) return kv_refuse("attn_packed: too many rows for one launch");
+    const uint32_t lds = (NW == 8 ? 3 * 3 * 64 : KG == 2 ? 3 * 64 : 3 * 32) * D * 2 + 16;
+    const int rl = kv_allow_lds(ctx, (const void *) k_attn_packed<O, D, PAGED, NW, KG>, lds, allowed);
     if (rl) return rl;
-    return emit(ctx, "attn_packed", k_attn_packed<O, D, PAGED>, dim3((uint32_t) blocks), dim3(512), lds, a);
+    return emit(ctx, "attn_packed", k_attn_packed<O, D, PAGED, NW, KG>, dim3((uint32_t) blocks), dim3(64 * NW), lds, a);
+}
+// Which form a call gets, by what the host knows (rows, sequences, an upper bound of the rows and of the keys of one); us for BF16, [sequences] x [rows]
+// (+ [keys before them]), [query heads]/[K/V heads]:
+//   few rows, workgroups of 16 rows no more than CUs, some hundred keys: attn_paged.hip's kernel, whose eight waves take the keys in turn
+//       1 x 5 + 8192, 32/8 of 128: 77 (143 here);  1 x 32 + 1500, 20/20 of 64: 13.5 (36);  but 32 x 8 + 1000, 32/8: 50 (29)
+//   64 dims: four waves, 128 rows (8 x 1500, 20/20: 101; eight waves 122); where that leaves CUs idle, 64 rows and two waves on each tile's keys
+//       (1 x 1500, 20/20: 25; 38.  1 x 4096, 20/20: 82; 100)
+//   128 dims: eight waves, 256 rows (1 x 8192, 32/8: 565; four waves 661).  Up to 768 keys the start and the end of a workgroup weigh more than its
+//       loop: four waves, two workgroups to a CU (64 x 128, 32/8: 51; 64.  32 x 512: 157; 167.  8 x 1024: 120; 118).  Few workgroups: two waves on each
+//       tile's keys (1 x 8192, 8/8, whose last rows' workgroups are twice the mean: 205; 250.  2 x 256 + 8192, 32/8: 177; 253), but not where that makes
+//       a second round of workgroups of equal length (4 x 512 + 2048 of a window, 32/8: 133; 96)
+template <typename O, int D, bool PAGED>
+static int launch_packed(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv, int max_q, int64_t keys) {
+    const int64_t rows = (int64_t) a.rows_q * a.G, per = (rows + a.n - 1) / a.n;     // rows (query x head of a group), and of one sequence on the average
+    const int64_t few = (int64_t) a.n * Hkv * ((max_q * (int64_t) a.G + 15) / 16);   // workgroups of 16 rows
+    if (max_q > 0 && (int64_t) max_q * a.G <= 256 && few <= ctx->n_cu && keys >= 256) return mi355x_attn_few_rows(ctx, a, __is_same(O, f16_ops) ? MI355X_TYPE_F16 : MI355X_TYPE_BF16, D, PAGED);
+    const int64_t wide = rows * Hkv / 256;                           // workgroups of 256 rows, if all were full
+    if constexpr (D == 64) {
+        if (wide < 512 && keys >= 128) return launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv);
+        return launch_packed_as<O, D, PAGED, 4, 1>(ctx, a, Hkv);
+    } else {
+        const bool wedge = a.causal && a.window == 0 && keys <= 2 * (a.rows_q / a.n);
+        if (wide <= (wedge ? ctx->n_cu : ctx->n_cu / 2) && keys >= 256) return per <= 64 ? launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv) : launch_packed_as<O, D, PAGED, 8, 2>(ctx, a, Hkv);
+        return keys <= 768 ? launch_packed_as<O, D, PAGED, 4, 1>(ctx, a, Hkv) : launch_packed_as<O, D, PAGED, 8, 1>(ctx, a, Hkv);
+    }
 }
 
 extern "C" int mi355x_attn_packed(mi355x_ctx * ctx, const mi355x_attn_packed_desc * d) {
@@ -382,12 +399,11 @@ extern "C" int mi355x_attn_packed(mi355x_ctx * ctx, const mi355x_attn_packed_des
     a.o = (char *) d->dst.data; a.o_nb1 = d->dst.nb[1]; a.o_nb2 = d->dst.nb[2]; a.o_type = d->dst.type;
     a.cu_q = d->cu_q; a.cu_k = d->cu_k ? d->cu_k : d->cu_q; a.seq = d->seq;
     a.c2 = fmaxf(fabsf(d->scale) * 1.4426950408889634f, 1e-37f); a.flip = d->scale < 0.0f; a.n = d->n; a.rows_q = (int) rows; a.causal = d->causal != 0; a.window = d->window;
-    a.G = (int) (H / Hkv); a.Hkv = (int) Hkv; a.qt = 256 / a.G;
-    const int64_t blocks = (rows / a.qt + d->n) * Hkv;
-    if (blocks > INT32_MAX) return kv_refuse("attn_packed: too many rows for one launch");
+    a.G = (int) (H / Hkv); a.Hkv = (int) Hkv;
     const bool f16 = type == MI355X_TYPE_F16, paged = d->cache != nullptr;
-    if (dim == 64) return f16 ? (paged ? launch_packed<f16_ops, 64, true>(ctx, a, blocks) : launch_packed<f16_ops, 64, false>(ctx, a, blocks))
-                              : (paged ? launch_packed<bf16_ops, 64, true>(ctx, a, blocks) : launch_packed<bf16_ops, 64, false>(ctx, a, blocks));
-    return f16 ? (paged ? launch_packed<f16_ops, 128, true>(ctx, a, blocks) : launch_packed<f16_ops, 128, false>(ctx, a, blocks))
-               : (paged ? launch_packed<bf16_ops, 128, true>(ctx, a, blocks) : launch_packed<bf16_ops, 128, false>(ctx, a, blocks));
+    const int64_t keys = paged ? (int64_t) d->cache->max_pages * d->cache->page_size : a.rows_k / d->n;       // of a sequence, as far as the host knows
+    if (dim == 64) return f16 ? (paged ? launch_packed<f16_ops, 64, true>(ctx, a, Hkv, d->max_q, keys) : launch_packed<f16_ops, 64, false>(ctx, a, Hkv, d->max_q, keys))
+                              : (paged ? launch_packed<bf16_ops, 64, true>(ctx, a, Hkv, d->max_q, keys) : launch_packed<bf16_ops, 64, false>(ctx, a, Hkv, d->max_q, keys));
+    return f16 ? (paged ? launch_packed<f16_ops, 128, true>(ctx, a, Hkv, d->max_q, keys) : launch_packed<f16_ops, 128, false>(ctx, a, Hkv, d->max_q, keys))
+               : (paged ? launch_packed<bf16_ops, 128, true>(ctx, a, Hkv, d->max_q, keys) : launch_packed<bf16_ops, 128, false>(ctx, a, Hkv, d->max_q, keys));
 }

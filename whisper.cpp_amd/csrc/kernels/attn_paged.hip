@@ -29,10 +29,14 @@ struct PagedArgs {
     int q_type, o_type, window;
     int G, H, groups;                  // query heads per K/V head, query heads, sets of 16 query heads per K/V head
     int shares, min_tiles;
+    const int * cu_q, * cu_k;          // packed rows: as in PackedArgs
+    int n, rows_q, rows_k, causal;
+    int qt, hg;                        // queries of a tile of 16 rows, heads of the group that each has there: qt * hg <= 16
 };
 
 // the keys that query i sees, as [lo, hi), and the tiles of one share
 struct paged_span { int s, lo, hi, per; };
+__device__ __forceinline__ int tiles_of(const paged_span & p) { return p.hi > p.lo ? (p.hi + TILE - 1) / TILE - p.lo / TILE : 0; }
 __device__ __forceinline__ paged_span span_of(const PagedArgs & a, int i) {
     paged_span r;
     r.s = a.seq ? a.seq[i] : i;
@@ -41,14 +45,11 @@ __device__ __forceinline__ paged_span span_of(const PagedArgs & a, int i) {
     const int64_t cap = (int64_t) a.c.max_pages << a.c.shift;
     r.hi = len < 0 ? 0 : len > cap ? (int) cap : len;
     r.lo = a.window > 0 && r.hi > a.window ? r.hi - a.window : 0;
-    const int tiles = r.hi > 0 ? (r.hi + TILE - 1) / TILE - r.lo / TILE : 0;
+    const int tiles = tiles_of(r);
     r.per = max((tiles + a.shares - 1) / a.shares, a.min_tiles);
     return r;
 }
-__device__ __forceinline__ int shares_of(const paged_span & p) {
-    const int tiles = p.hi > 0 ? (p.hi + TILE - 1) / TILE - p.lo / TILE : 0;
-    return (tiles + p.per - 1) / p.per;
-}
+__device__ __forceinline__ int shares_of(const paged_span & p) { return (tiles_of(p) + p.per - 1) / p.per; }
 
 // F32 values as NT terms of a 16-bit type: x = t0 + t1 (+ t2), each the rounding of what the ones before leave
 template <typename O, int NT> __device__ __forceinline__ void split8(const float * f, typename O::vec8 * t) {
@@ -65,7 +66,9 @@ template <int D> __device__ __forceinline__ int v_piece(int key, int piece) {
     return D == 128 ? piece ^ ((key & 7) << 1) : piece ^ (((key >> 1) & 3) << 1);
 }
 
-template <typename O, int D, int NT, bool BIG>           // BIG: pages of 32 keys and more: a tile lies in one page
+enum { SMALL_PAGES, BIG_PAGES, ROWS };                   // where K and V lie: pages of fewer than 32 keys; 32 and more (a tile lies in one); packed rows
+
+template <typename O, int D, int NT, int SRC, bool PACKED>
 __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     typedef typename O::vec8 vec8;
     constexpr int KK = D / 32;                           // 32-dim pieces of a key
@@ -73,19 +76,45 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     constexpr int RPL = 512 / D;                         // V rows per load
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, nl = lane & 15, g4 = lane >> 4, waves = blockDim.x >> 6;
-    const int unit = blockIdx.x, grp = unit % a.groups, hk = unit / a.groups % a.c.Hkv, i = unit / a.groups / a.c.Hkv, share = blockIdx.y;
-    const paged_span sp = span_of(a, i);
-    const int t0 = sp.lo / TILE + share * sp.per, t1 = min(t0 + sp.per, (sp.hi + TILE - 1) / TILE);
-    const int g0 = grp * 16, rows = min(16, a.G - g0), h0 = hk * a.G + g0;
+    const int unit = blockIdx.x, grp = unit % a.groups, hk = unit / a.groups % a.c.Hkv, share = blockIdx.y;
+    int i = unit / a.groups / a.c.Hkv;                   // the query; packed: the first query row of this workgroup
+    paged_span sp;
+    int nq = 1, k0 = 0, own = 0;                         // packed: queries here, the keys' first row, the first query's own key
+    if (PACKED) {
+        packed_job job;
+        if (!packed_find(a, i, job)) return;
+        int L = 0;
+        sp.s = -1;
+        if (SRC == ROWS) {
+            k0 = a.cu_k[job.i]; const int k1 = a.cu_k[job.i + 1];
+            if (k0 >= 0 && k1 <= a.rows_k && k1 > k0) L = k1 - k0;
+        } else {
+            sp.s = a.seq ? a.seq[job.i] : job.i;
+            if (sp.s >= 0 && sp.s < a.c.n_seq) { const int64_t cap = (int64_t) a.c.max_pages << a.c.shift; const int len = a.c.len[sp.s]; L = len < 0 ? 0 : len > cap ? (int) cap : len; }
+        }
+        const int q0 = job.tile * a.qt;
+        nq = min(a.qt, job.nq - q0); own = L - job.nq + q0; i = job.r0 + q0;
+        sp.lo = a.window > 0 ? max(own - a.window + 1, 0) : 0;
+        sp.hi = a.causal ? min(own + nq, L) : L;
+        sp.per = 1 << 30;
+    } else sp = span_of(a, i);
+    const int t0 = sp.lo / TILE + share * sp.per, t1 = tiles_of(sp) ? min(t0 + sp.per, (sp.hi + TILE - 1) / TILE) : t0;
+    const int g0 = grp * 16, rows = PACKED ? nq * a.hg : min(16, a.G - g0), h0 = hk * a.G + g0;
     if (t0 >= t1 && (share > 0 || a.shares > 1)) return;             // (an empty sequence: k_attn_join writes its zeros, or this workgroup below)
     char * vl = lds + wave * (TILE * D * 2);
+    // row r of the 16: query i + r / hg, head h0 + r % hg (one query: head h0 + r).  The keys that lane nl's row sees are first .. last.
+    auto q_of = [&](int r) { return PACKED ? r / a.hg : 0; };
+    auto h_of = [&](int r) { return PACKED ? r - r / a.hg * a.hg : r; };
+    const bool here = nl < rows && g0 + h_of(nl) < a.G;
+    const int ql = min(q_of(nl), nq - 1);
+    const int last = PACKED && a.causal ? min(own + ql, sp.hi - 1) : sp.hi - 1, first = PACKED && a.window > 0 ? max(own + ql - a.window + 1, 0) : sp.lo;
 
     // Q^T as the second operand: lane (head nl, dims 32 kk + 8 g4 ..)
     vec8 qf[NT][KK];
     #pragma unroll
     for (int kk = 0; kk < KK; kk++) {
         float f[8] = { 0, 0, 0, 0, 0, 0, 0, 0 };
-        if (nl < rows) load8(a.q + (int64_t) i * a.q_nb2 + (int64_t) (h0 + nl) * a.q_nb1 + (32 * kk + 8 * g4) * (a.q_type == MI355X_TYPE_F32 ? 4 : 2), a.q_type, f);
+        if (here) load8(a.q + (int64_t) (i + q_of(nl)) * a.q_nb2 + (int64_t) (h0 + h_of(nl)) * a.q_nb1 + (32 * kk + 8 * g4) * (a.q_type == MI355X_TYPE_F32 ? 4 : 2), a.q_type, f);
         vec8 t[NT];
         split8<O, NT>(f, t);
         #pragma unroll
@@ -96,18 +125,23 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     // the page of each key of a tile, in lane key & 31.  Keys outside the span are replaced by the nearest inside: what no row sees is not read.
     bool bad = false;
     auto pages_of = [&](int t) {
+        if (SRC == ROWS) return 0;
         const int key = min(max(t * TILE + (lane & 31), sp.lo), sp.hi - 1);
         int p = row[key >> a.c.shift];
         bad |= (unsigned) p >= (unsigned) a.c.n_pages;
         return min(max(p, 0), a.c.n_pages - 1);
+    };
+    auto place = [&](int key, int kl, int pg) -> int64_t {           // kl: the key's number in the tile
+        if (SRC == ROWS) return (int64_t) (k0 + key) * a.c.nb_key;
+        const int p = SRC == BIG_PAGES ? __builtin_amdgcn_readfirstlane(pg) : __shfl(pg, kl, 64);
+        return p * a.c.nb_page + (key & a.c.mask) * a.c.nb_key;
     };
     vec8 kr[2][KK]; u32x4_t vr[NV];
     auto fetch_k = [&](int t, int pg) {
         #pragma unroll
         for (int b = 0; b < 2; b++) {
             const int key = min(max(t * TILE + 16 * b + nl, sp.lo), sp.hi - 1);
-            const int p = BIG ? __builtin_amdgcn_readfirstlane(pg) : __shfl(pg, 16 * b + nl, 64);
-            const char * at = kb + p * a.c.nb_page + (key & a.c.mask) * a.c.nb_key + 16 * g4;
+            const char * at = kb + place(key, 16 * b + nl, pg) + 16 * g4;
             #pragma unroll
             for (int kk = 0; kk < KK; kk++) kr[b][kk] = *(const vec8 *) (at + 64 * kk);
         }
@@ -116,8 +150,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
         #pragma unroll
         for (int r = 0; r < NV; r++) {
             const int kl = r * RPL + lane / (D / 8), key = min(max(t * TILE + kl, sp.lo), sp.hi - 1);
-            const int p = BIG ? __builtin_amdgcn_readfirstlane(pg) : __shfl(pg, kl, 64);
-            vr[r] = *(const u32x4_t *) (vb + p * a.c.nb_page + (key & a.c.mask) * a.c.nb_key + (lane % (D / 8)) * 16);
+            vr[r] = *(const u32x4_t *) (vb + place(key, kl, pg) + (lane % (D / 8)) * 16);
         }
     };
 
@@ -143,12 +176,26 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
                     for (int kk = 0; kk < KK; kk++) s[b] = O::mfma16(kr[b][kk], qf[n][kk], s[b]);
             }
             if (more) fetch_k(t + waves, pg);
-            #pragma unroll
-            for (int r = 0; r < NV; r++) {
-                const int kl = r * RPL + lane / (D / 8);
-                *(u32x4_t *) (vl + kl * (D * 2) + v_piece<D>(kl, lane % (D / 8)) * 16) = vr[r];
+            // V into this wave's area.  Zero times an infinity or a NaN is none: where some row does not see all of the tile, they are taken out here,
+            // and counted over the keys that each row sees below (rare: the next V tile waits for it).
+            bool odd = false;
+            if (PACKED && (t * TILE + TILE - 1 > (a.causal ? own : sp.hi - 1) || (a.window > 0 && t * TILE < own + nq - a.window))) {
+                uint32_t nf = 0;
+                #pragma unroll
+                for (int r = 0; r < NV; r++) nf |= not_finite8<O>(vr[r]);
+                odd = __any(nf != 0);
             }
-            if (more) {
+            auto put_v = [&](int what) {                             // 0: as it is, 1: without what is not finite, 2: what that was
+                #pragma unroll
+                for (int r = 0; r < NV; r++) {
+                    const int kl = r * RPL + lane / (D / 8);
+                    u32x4_t x = vr[r], kind = { 0, 0, 0, 0 };
+                    if (what) take_apart<O>(x, kind);
+                    *(u32x4_t *) (vl + kl * (D * 2) + v_piece<D>(kl, lane % (D / 8)) * 16) = what == 2 ? kind : x;
+                }
+            };
+            if (PACKED && odd) put_v(1); else put_v(0);
+            if (more && !odd) {
                 fetch_v(t + waves, pg);
                 pg = pages_of(min(t + 2 * waves, t1 - 1));
             }
@@ -157,7 +204,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
             #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int key = t * TILE + 16 * (e >> 2) + 4 * g4 + (e & 3);
-                x[e] = key >= sp.lo && key < sp.hi ? s[e >> 2][e & 3] * a.c2 : -INFINITY;
+                x[e] = key >= first && key <= last ? s[e >> 2][e & 3] * a.c2 : -INFINITY;
                 top = fmaxf(top, x[e]);
             }
             top = fmaxf(top, lane_xor16(top));
@@ -177,9 +224,8 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
             for (int e = 0; e < 8; e++) { p[e] = __builtin_amdgcn_exp2f(x[e] - shift); l += p[e]; }
             vec8 pf[NT];
             split8<O, NT>(p, pf);
-            #pragma unroll
-            for (int d = 0; d < NV; d++) {
-                // V^T as the first operand: this 16-lane group's keys 4 g4 + {0..3} and 16 + 4 g4 + {0..3}, dims 16 d + {0..15}
+            // V^T as the first operand: this 16-lane group's keys 4 g4 + {0..3} and 16 + 4 g4 + {0..3}, dims 16 d + {0..15}
+            auto v_frag = [&](int d) {
                 vec8 vf;
                 #pragma unroll
                 for (int b = 0; b < 2; b++) {
@@ -188,12 +234,36 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
                     const short4_t r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *) at);
                     __builtin_memcpy((char *) &vf + 8 * b, &r, 8);
                 }
+                return vf;
+            };
+            #pragma unroll
+            for (int d = 0; d < NV; d++) {
+                const vec8 vf = v_frag(d);
                 #pragma unroll
                 for (int n = NT - 1; n >= 0; n--) o[d] = O::mfma16(vf, pf[n], o[d]);
             }
+            if (PACKED && odd) {
+                put_v(2);
+                vec8 seen;
+                #pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = t * TILE + 16 * (e >> 2) + 4 * g4 + (e & 3);
+                    seen[e] = (typename O::elem) (key >= first && key <= last ? 1.0f : 0.0f);
+                }
+                #pragma unroll
+                for (int d = 0; d < NV; d++) {
+                    const floatx4 cnt = O::mfma16(v_frag(d), seen, floatx4{ 0, 0, 0, 0 });
+                    #pragma unroll
+                    for (int r = 0; r < 4; r++) o[d][r] += put_back(cnt[r]);
+                }
+                if (more) {
+                    fetch_v(t + waves, pg);
+                    pg = pages_of(min(t + 2 * waves, t1 - 1));
+                }
+            }
         }
     }
-    if (__any(bad) && lane == 0) atomicOr((unsigned *) a.c.status, MI355X_KV_BAD_ARG);
+    if (SRC != ROWS && __any(bad) && lane == 0) atomicOr((unsigned *) a.c.status, MI355X_KV_BAD_ARG);
     l += lane_xor16(l);
     l += lane_xor32(l);
 
@@ -206,6 +276,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     __syncthreads();
     for (int j = threadIdx.x; j < rows * (D / 4); j += blockDim.x) {
         const int h = j / (D / 4), d = j % (D / 4) * 4;
+        if (PACKED && g0 + h_of(h) >= a.G) continue;
         float M = NEG_BIG, L = 0.0f;
         for (int w = 0; w < waves; w++) M = fmaxf(M, ml[w * 32 + h]);
         floatx4 r = { 0, 0, 0, 0 };
@@ -218,7 +289,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
         }
         if (a.shares == 1) {
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            store4(a.o + (int64_t) i * a.o_nb2 + (int64_t) (h0 + h) * a.o_nb1 + d * (a.o_type == MI355X_TYPE_F32 ? 4 : 2), a.o_type, r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
+            store4(a.o + (int64_t) (i + q_of(h)) * a.o_nb2 + (int64_t) (h0 + h_of(h)) * a.o_nb1 + d * (a.o_type == MI355X_TYPE_F32 ? 4 : 2), a.o_type, r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
         } else {
             const int64_t rec = ((int64_t) i * a.H + h0 + h) * a.shares + share;
             *(floatx4 *) (a.part_o + rec * D + d) = r;
@@ -283,16 +354,35 @@ extern "C" size_t mi355x_attn_paged_work_bytes(const mi355x_kv_cache * c, int n,
     return s == 1 ? 0 : (size_t) n * n_head * s * (c->head_dim + 2) * 4;
 }
 
-template <typename O, int D, int NT>
-static int launch_paged(mi355x_ctx * ctx, const PagedArgs & a, int n, int threads, double bytes, double flops) {
-    const dim3 grid((uint32_t) ((int64_t) n * a.c.Hkv * a.groups), (uint32_t) a.shares), block(threads);
+template <typename O, int D, int NT, int SRC, bool PACKED>
+static int launch_as(mi355x_ctx * ctx, const PagedArgs & a, int64_t blocks, int threads) {
     const uint32_t v = (uint32_t) (threads / 64 * TILE * D * 2), j = (uint32_t) (threads / 64 * (32 + 16 * (D + 4)) * 4), lds = v > j ? v : j;
-    const bool big = a.c.shift >= 5;
-    const void * f = big ? (const void *) k_attn_paged<O, D, NT, true> : (const void *) k_attn_paged<O, D, NT, false>;
-    static std::atomic<uint64_t> allowed[2];
-    const int rl = kv_allow_lds(ctx, f, lds, allowed[big]);
-    if (rl) return rl;
-    return mi355x_emit(ctx, "attn_paged", f, grid, block, lds, &a, sizeof(a), bytes, flops);
+    static std::atomic<uint64_t> allowed{0};
+    const int rl = kv_allow_lds(ctx, (const void *) k_attn_paged<O, D, NT, SRC, PACKED>, lds, allowed);
+    return rl ? rl : emit(ctx, PACKED ? "attn_packed" : "attn_paged", k_attn_paged<O, D, NT, SRC, PACKED>, dim3((uint32_t) blocks, (uint32_t) a.shares), dim3(threads), lds, a);
+}
+template <typename O, int D, int NT>
+static int launch_paged(mi355x_ctx * ctx, const PagedArgs & a, int n, int threads) {
+    const int64_t blocks = (int64_t) n * a.c.Hkv * a.groups;
+    return a.c.shift >= 5 ? launch_as<O, D, NT, BIG_PAGES, false>(ctx, a, blocks, threads) : launch_as<O, D, NT, SMALL_PAGES, false>(ctx, a, blocks, threads);
+}
+template <typename O, int D>
+static int launch_few(mi355x_ctx * ctx, const PagedArgs & a, bool paged) {
+    const int64_t blocks = ((int64_t) a.rows_q / a.qt + a.n) * a.c.Hkv * a.groups;
+    if (blocks > INT32_MAX) return kv_refuse("attn_packed: too many rows for one launch");
+    if (!paged) return launch_as<O, D, 1, ROWS, true>(ctx, a, blocks, 512);
+    return a.c.shift >= 5 ? launch_as<O, D, 1, BIG_PAGES, true>(ctx, a, blocks, 512) : launch_as<O, D, 1, SMALL_PAGES, true>(ctx, a, blocks, 512);
+}
+int mi355x_attn_few_rows(mi355x_ctx * ctx, const PackedArgs & p, int type, int dim, bool paged) {
+    PagedArgs a; memset(&a, 0, sizeof(a));
+    a.c = p.c; a.c.Hkv = p.Hkv; a.seq = p.seq;
+    a.q = p.q; a.q_nb1 = p.q_nb1; a.q_nb2 = p.q_nb2; a.q_type = p.q_type;
+    a.o = p.o; a.o_nb1 = p.o_nb1; a.o_nb2 = p.o_nb2; a.o_type = p.o_type;
+    a.c2 = p.flip ? -p.c2 : p.c2; a.window = p.window; a.G = p.G; a.H = p.G * p.Hkv; a.groups = (p.G + 15) / 16; a.shares = 1; a.min_tiles = 1 << 30;
+    a.cu_q = p.cu_q; a.cu_k = p.cu_k; a.n = p.n; a.rows_q = p.rows_q; a.rows_k = p.rows_k; a.causal = p.causal;
+    a.hg = p.G < 16 ? p.G : 16; a.qt = 16 / a.hg;
+    if (dim == 64) return type == MI355X_TYPE_F16 ? launch_few<f16_ops, 64>(ctx, a, paged) : launch_few<bf16_ops, 64>(ctx, a, paged);
+    return type == MI355X_TYPE_F16 ? launch_few<f16_ops, 128>(ctx, a, paged) : launch_few<bf16_ops, 128>(ctx, a, paged);
 }
 
 extern "C" int mi355x_attn_paged(mi355x_ctx * ctx, const mi355x_kv_cache * c, const mi355x_attn_paged_desc * d) {
@@ -324,10 +414,10 @@ extern "C" int mi355x_attn_paged(mi355x_ctx * ctx, const mi355x_kv_cache * c, co
     const int threads = a.shares == 1 ? 512 : 256;
     const bool f16 = c->type == MI355X_TYPE_F16, one = d->q.type == c->type;
     int e;
-    if (c->head_dim == 64) e = f16 ? (one ? launch_paged<f16_ops, 64, 1>(ctx, a, (int) n, threads, 0, 0) : launch_paged<f16_ops, 64, 2>(ctx, a, (int) n, threads, 0, 0))
-                                   : (one ? launch_paged<bf16_ops, 64, 1>(ctx, a, (int) n, threads, 0, 0) : launch_paged<bf16_ops, 64, 3>(ctx, a, (int) n, threads, 0, 0));
-    else                   e = f16 ? (one ? launch_paged<f16_ops, 128, 1>(ctx, a, (int) n, threads, 0, 0) : launch_paged<f16_ops, 128, 2>(ctx, a, (int) n, threads, 0, 0))
-                                   : (one ? launch_paged<bf16_ops, 128, 1>(ctx, a, (int) n, threads, 0, 0) : launch_paged<bf16_ops, 128, 3>(ctx, a, (int) n, threads, 0, 0));
+    if (c->head_dim == 64) e = f16 ? (one ? launch_paged<f16_ops, 64, 1>(ctx, a, (int) n, threads) : launch_paged<f16_ops, 64, 2>(ctx, a, (int) n, threads))
+                                   : (one ? launch_paged<bf16_ops, 64, 1>(ctx, a, (int) n, threads) : launch_paged<bf16_ops, 64, 3>(ctx, a, (int) n, threads));
+    else                   e = f16 ? (one ? launch_paged<f16_ops, 128, 1>(ctx, a, (int) n, threads) : launch_paged<f16_ops, 128, 2>(ctx, a, (int) n, threads))
+                                   : (one ? launch_paged<bf16_ops, 128, 1>(ctx, a, (int) n, threads) : launch_paged<bf16_ops, 128, 3>(ctx, a, (int) n, threads));
     if (e || a.shares == 1) return e;
     const dim3 grid((uint32_t) (n * H));
     return c->head_dim == 64 ? emit(ctx, "attn_join", k_attn_join<64>, grid, dim3(256), 0, a) : emit(ctx, "attn_join", k_attn_join<128>, grid, dim3(256), 0, a);

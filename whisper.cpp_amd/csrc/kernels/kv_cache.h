@@ -1,6 +1,7 @@
 // Internal header of the paged K/V cache: what kv_cache.hip, attn_paged.hip and attn_packed.hip share.
 #pragma once
 #include "common.h"
+#include <math.h>
 #include <atomic>
 
 // the calling thread's device is the context's for the length of a call, and the caller's again afterwards
@@ -60,6 +61,10 @@ static inline int kv_allow_lds(mi355x_ctx * ctx, const void * f, uint32_t lds, s
 }
 
 #ifdef __HIPCC__
+struct PackedArgs;
+// attn_paged.hip: packed sequences of few rows (up to 16 rows of a K/V head at a time, every wave its own tiles of the keys)
+int mi355x_attn_few_rows(mi355x_ctx * ctx, const PackedArgs & a, int type, int dim, bool paged);
+
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef short  short4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
@@ -98,4 +103,64 @@ __device__ __forceinline__ void store4(char * p, int type, float a, float b, flo
     else if (type == MI355X_TYPE_F16) { half4_t h; h[0] = (half_t) a; h[1] = (half_t) b; h[2] = (half_t) c; h[3] = (half_t) d; *(half4_t *) p = h; }
     else { typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4))); bf16x4_t h; h[0] = (__bf16) a; h[1] = (__bf16) b; h[2] = (__bf16) c; h[3] = (__bf16) d; *(bf16x4_t *) p = h; }
 }
+
+// ---- packed rows (attn_packed.hip, and attn_paged.hip's kernel for few rows) ----
+struct PackedArgs {
+    kvc c;                             // PAGED: the cache.  Otherwise k, v and their strides in nb_key (rows) and nb_head
+    const char * q; int64_t q_nb1, q_nb2;
+    char * o; int64_t o_nb1, o_nb2;
+    const int * cu_q, * cu_k, * seq;
+    float c2; int flip;                // |scale| * log2(e), at least 1e-37; whether the scale is negative (the queries change sign)
+    int n, rows_q, rows_k, q_type, o_type, causal, window;
+    int G, Hkv, qt;                    // query heads per K/V head; queries of a workgroup
+};
+
+// slot -> (sequence, tile of its rows): sequence i has the slots cu[i]/qt + i .. cu[i+1]/qt + i, at least as many as its tiles.  A wave looks at 64
+// sequences at a time: one load's latency where a bisection has log2(n) of them.
+struct packed_job { int i, r0, nq, tile; };
+template <typename A> __device__ __forceinline__ bool packed_find(const A & a, int slot, packed_job & j) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, step = 1;
+    while (step * 64 < a.n) step *= 64;                              // coarse to fine: every `step`-th sequence behind lo
+    for (; step > 0; step /= 64) {
+        const int i = (int) min((int64_t) lo + (int64_t) lane * step, (int64_t) a.n);
+        const unsigned long long m = __ballot(i < a.n && a.cu_q[i] / a.qt + i <= slot);
+        lo += max(__popcll(m) - 1, 0) * step;
+    }
+    j.i = lo;
+    j.r0 = a.cu_q[lo]; const int r1 = a.cu_q[lo + 1];
+    if (j.r0 < 0 || r1 > a.rows_q || r1 <= j.r0) return false;
+    j.nq = r1 - j.r0;
+    const int tiles = (j.nq + a.qt - 1) / a.qt, t = slot - (j.r0 / a.qt + lo);
+    if (t < 0 || t >= tiles) return false;
+    j.tile = tiles - 1 - t;                                          // the rows with most keys first
+    return true;
+}
+
+// bit 15 of each half: whether it is an infinity or a NaN
+template <typename O> __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
+    return ((w & 0x7FFF7FFFu) + (__is_same(O, f16_ops) ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+template <typename O> __device__ __forceinline__ uint32_t not_finite8(u32x4_t w) { return not_finite2<O>(w[0]) | not_finite2<O>(w[1]) | not_finite2<O>(w[2]) | not_finite2<O>(w[3]); }
+
+// infinities and NaNs out of eight values: zeros in their places, and what they were as numbers of the type: 1 (inf), 128 (-inf), 16384 (NaN)
+template <typename O> __device__ __forceinline__ void take_apart(u32x4_t & v, u32x4_t & kind) {
+    constexpr bool F = __is_same(O, f16_ops);
+    #pragma unroll
+    for (int w = 0; w < 4; w++)
+        #pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+            const uint32_t x = v[w] >> h & 0xFFFF, top = F ? 0x7C00 : 0x7F80;
+            if ((x & top) != top) continue;
+            kind[w] |= ((x & 0x7FFF) != top ? (F ? 0x7400u : 0x4680u) : x & 0x8000 ? (F ? 0x5800u : 0x4300u) : (F ? 0x3C00u : 0x3F80u)) << h;
+            v[w] &= ~(0xFFFFu << h);
+        }
+}
+
+// what a count over visible keys of the numbers above adds to a sum (at most 64 of each kind)
+__device__ __forceinline__ float put_back(float count) {
+    const int n = (int) count;
+    return ((n & 127) ? INFINITY : 0.0f) + ((n & 0x3F80) ? -INFINITY : 0.0f) + (n >= 16384 ? NAN : 0.0f);
+}
+
 #endif
