@@ -18,8 +18,6 @@
 // what a 16-byte piece's number in its row is changed by (exclusive-or): the rows that an instruction reads together lie in different banks
 template <int D> __device__ __forceinline__ int k_swap(int key) { return D == 128 ? key & 15 : key >> 1 & 7; }
 template <int D> __device__ __forceinline__ int v_swap(int key) { return D == 128 ? (key & 3) << 2 : (key >> 1 & 1) << 2; }
-#define LDS __attribute__((address_space(3)))
-__device__ __forceinline__ uint32_t lds_at(char * p) { return (uint32_t) (size_t) (LDS char *) p; }
 
 template <typename O, int D, bool PAGED, int NW, int KG>
 __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) {

@@ -83,6 +83,10 @@ struct bf16_ops {
     static __device__ __forceinline__ floatx16 mfma32(vec8 a, vec8 b, floatx16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 
+// LDS by its 32-bit address
+#define LDS __attribute__((address_space(3)))
+__device__ __forceinline__ uint32_t lds_at(char * p) { return (uint32_t) (size_t) (LDS char *) p; }
+
 // eight consecutive elements of F32 / F16 / BF16 memory as floats, and back
 __device__ __forceinline__ void load8(const char * p, int type, float * f) {
     if (type == MI355X_TYPE_F32) {
