@@ -344,6 +344,40 @@ def test_attention_of_one_token_split_over_a_long_cache_and_joined(gpu, n, lengt
         same(torch, rows[0][s], o, tol)
 
 
+@pytest.mark.parametrize("kind,q_kind,dim,kv_heads,heads,page,window", [("f16", "f16", 64, 1, 3, 16, 0), ("bf16", "f32", 128, 2, 4, 64, 0), ("bf16", "bf16", 128, 1, 17, 8, 700)])
+def test_many_queries_of_very_different_lengths_share_the_runs_of_the_split(gpu, kind, q_kind, dim, kv_heads, heads, page, window):
+    """hundreds of queries, most of them short, some empty or left out, a few long: runs that hold several, that begin and end inside one"""
+    ctx, ka, torch = gpu
+    rng, gen, n = random.Random(7), torch.Generator(device="cuda").manual_seed(4), 200
+    lens = [rng.choice((0, 1, 5, 31, 32, 33, 100, 300)) for _ in range(n)]
+    for i, x in zip(rng.sample(range(n), 5), (2900, 4100, 1500, 1025, 4097)):
+        lens[i] = x
+    held = [-(-x // page) for x in lens]
+    k, v = (torch.randn(sum(held), kv_heads, page, dim, generator=gen, device="cuda").to(dt(torch, kind)) for _ in range(2))
+    table, at = torch.full((n, max(held)), -1, dtype=torch.int32), 0
+    for s, h in enumerate(held):
+        table[s, :h] = torch.arange(at, at + h)
+        at += h
+    zero = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+    work, status, dtab, dlen, ref = torch.empty(ka.kv_work_bytes(n, sum(held)), dtype=torch.uint8, device="cuda"), zero(1), table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), zero(sum(held))
+    c = ka.kv_cache(k, v, dtab, dlen, ref, status, work)
+    seq = rng.sample(range(n), n) + [-1, 0, 0, n + 5]
+    q = torch.randn(len(seq), heads, dim, generator=gen, device="cuda").to(dt(torch, q_kind))
+    out, space, scale = torch.full_like(q, 3.0), torch.full((ka.attn_paged_work_bytes(c, len(seq), heads),), 255, dtype=torch.uint8, device="cuda"), 1 / math.sqrt(dim)
+    assert space.numel() > 0
+    dseq = torch.tensor(seq, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    ctx.attn_paged_call(c, q, out, seq=dseq, scale=scale, window=window, work=space)()
+    ctx.sync()
+    assert int(status) == 0
+    for i in sorted(rng.sample(range(len(seq)), 60) + [j for j, s in enumerate(seq) if not 0 <= s < n or lens[s] > 1000]):
+        s = seq[i] if 0 <= seq[i] < n else None
+        L = lens[s] if s is not None else 0
+        flat = [x.cpu()[table[s, : held[s]].long()].transpose(1, 2).reshape(-1, kv_heads, dim)[:L] if L else torch.zeros(0, kv_heads, dim) for x in (k, v)]
+        o, tol = expect(torch, q[i].cpu(), *flat, torch.arange(L) >= (L - window if window else 0), scale, kind, q_kind, q_kind, False, q_kind == kind)
+        same(torch, out[i], o, tol)
+
+
 def packed_case(gpu, kind, q_kind, out_kind, dim, kv_heads, heads, q_lens, k_lens=None, window=0, causal=True, page=0, order="head", spoil=None, max_q=0, scale=None):
     """one call of the packed attention over rows of its own (page 0) or over a cache, against the definition.  `spoil`: {(sequence, key): (k, v)}"""
     ctx, ka, torch = gpu

@@ -87,32 +87,43 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
         for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    // staging: thread -> key tid / PCS (+ RPL), piece tid % PCS.  Keys outside what the workgroup sees are replaced by the nearest inside: never read.
+    // staging: thread -> key tid / PCS (+ RPL), piece tid % PCS.  A tile's keys behind the last are other rows of the pool or the last row again: no
+    // row sees them, and what of their values is not finite is taken out below.  A tile's places are made once, for its keys, and kept for its values.
     const int skey = tid / PCS, spc = tid % PCS;
     const char * kb = a.c.k + hk * a.c.nb_head + spc * 16, * vb = a.c.v + hk * a.c.nb_head + spc * 16;
+    if (!PAGED) { kb += k0 * a.c.nb_key; vb += k0 * a.c.nb_key; }
     bool bad = false;
     u32x4_t kr[NL], vr[NL];
-    int pg_k[NL], pg_v[NL], pg_n[NL];                                 // pages of the K tile and of the V tile that are fetched next, and of the tile behind
-    auto key_of = [&](int t, int e) { return min(max((T0 + t) * KT + skey + e * RPL, b_first), b_last); };
-    auto page_of = [&](int t, int * pg) {
+    int pg[NL];                                                       // pages of the tile whose places are made next
+    int64_t at_k[NL], at_v[NL];                                       // places of the K tile and of the V tile that are fetched next
+    const uint32_t nb_key = (uint32_t) a.c.nb_key, nb_page = (uint32_t) a.c.nb_page;
+    auto ask = [&](int t) {
         if (PAGED) {
             #pragma unroll
-            for (int e = 0; e < NL; e++) pg[e] = row[key_of(t, e) >> a.c.shift];
+            for (int e = 0; e < NL; e++) pg[e] = row[min(((T0 + t) * KT + skey + e * RPL) >> a.c.shift, a.c.max_pages - 1)];
         }
     };
-    auto place = [&](int t, int e, const int * pg) -> int64_t {
-        const int key = key_of(t, e);
-        if (!PAGED) return (int64_t) (k0 + key) * a.c.nb_key;
-        bad |= (unsigned) pg[e] >= (unsigned) a.c.n_pages;
-        return min(max(pg[e], 0), a.c.n_pages - 1) * a.c.nb_page + (key & a.c.mask) * a.c.nb_key;
-    };
-    auto fetch_k = [&](int t, const int * pg) {
+    auto make = [&](int t) {
         #pragma unroll
-        for (int e = 0; e < NL; e++) kr[e] = *(const u32x4_t *) (kb + place(t, e, pg));
+        for (int e = 0; e < NL; e++) {
+            const int key = (T0 + t) * KT + skey + e * RPL;
+            if (PAGED) {
+                bad |= (unsigned) pg[e] >= (unsigned) a.c.n_pages && key <= b_last;
+                at_k[e] = (int64_t) ((uint64_t) (uint32_t) min(max(pg[e], 0), a.c.n_pages - 1) * nb_page + (uint64_t) (uint32_t) (key & a.c.mask) * nb_key);
+            } else at_k[e] = (int64_t) ((uint64_t) (uint32_t) min(key, L - 1) * nb_key);
+        }
     };
-    auto fetch_v = [&](int t, const int * pg) {
+    auto keep = [&]() {
         #pragma unroll
-        for (int e = 0; e < NL; e++) vr[e] = *(const u32x4_t *) (vb + place(t, e, pg));
+        for (int e = 0; e < NL; e++) at_v[e] = at_k[e];
+    };
+    auto fetch_k = [&]() {
+        #pragma unroll
+        for (int e = 0; e < NL; e++) kr[e] = *(const u32x4_t *) (kb + at_k[e]);
+    };
+    auto fetch_v = [&](const int64_t * at) {
+        #pragma unroll
+        for (int e = 0; e < NL; e++) vr[e] = *(const u32x4_t *) (vb + at[e]);
     };
     const int k_put = skey * (D * 2) + (spc ^ k_swap<D>(skey)) * 16, v_put = skey * (D * 2) + (spc ^ v_swap<D>(skey)) * 16;     // (the same for keys RPL apart)
     auto put_k = [&](int t) {
@@ -256,26 +267,23 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
         // workgroup of the CU fills the gaps.
         const bool second = NW == 8 && wave >= 4;
         if (tid < SLOTS) odd[tid] = 0;
-        page_of(0, pg_k);
-        page_of(min(1, T - 1), pg_n);
-        fetch_k(0, pg_k);
-        if (VA == 1) fetch_v(0, pg_k);
+        ask(0); make(0);
+        ask(min(1, T - 1));
+        fetch_k();
+        if (VA == 1) fetch_v(at_k);
         put_k(0);
+        keep(); make(min(1, T - 1));
         if (KA == 2) {
-            fetch_k(min(1, T - 1), pg_n);
+            ask(min(2, T - 1));
+            fetch_k();
             __syncthreads();                                          // odd[] cleared
             put_v(0);
             put_k(1);
-            #pragma unroll
-            for (int e = 0; e < NL; e++) { pg_v[e] = pg_n[e]; }
-            page_of(min(2, T - 1), pg_k);
-        } else {
-            #pragma unroll
-            for (int e = 0; e < NL; e++) { pg_v[e] = pg_k[e]; pg_k[e] = pg_n[e]; }
+            keep(); make(min(2, T - 1));
         }
-        fetch_v(min(VA, T - 1), pg_v);                                // V tile VA, K tile KA next
-        fetch_k(min(KA, T - 1), pg_k);
-        page_of(min(KA + 1, T - 1), pg_n);
+        ask(min(KA + 1, T - 1));
+        fetch_v(at_v);                                                // V tile VA, K tile KA next
+        fetch_k();
         __syncthreads();
         if (second) __syncthreads();
         for (int t = 0; t < T; t++) {
@@ -286,13 +294,20 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
             __syncthreads();
             if (t + KA < T) put_k(t + KA);
             if (t + VA < T) put_v(t + VA);
+            // the places of K's tile of the step before are V's now.  Pages: the next places first, for a wait for the page numbers behind the loads of V
+            // would be one for those (piece over a cache: 90 us, so 80).  Rows: no such wait, and no copy of the places (long, grouped: 558 us, so 546)
+            if (PAGED) {
+                keep();
+                if (t + KA + 1 < T) make(t + KA + 1);
+                if (t + VA + 1 < T) fetch_v(at_v);
+            } else {
+                if (t + VA + 1 < T) fetch_v(at_k);
+                if (t + KA + 1 < T) make(t + KA + 1);
+            }
             if (t + KA + 1 < T) {
-                #pragma unroll
-                for (int e = 0; e < NL; e++) { pg_v[e] = pg_k[e]; pg_k[e] = pg_n[e]; }
-                fetch_k(t + KA + 1, pg_k);
-                page_of(min(t + KA + 2, T - 1), pg_n);
-                fetch_v(t + VA + 1, pg_v);
-            } else if (t + VA + 1 < T) fetch_v(t + VA + 1, pg_k);
+                fetch_k();
+                ask(min(t + KA + 2, T - 1));
+            }
             if (t >= t_lo && t < t_hi) softmax(t);
             if (!second || t + 1 < T) __syncthreads();
         }
@@ -383,6 +398,7 @@ extern "C" int mi355x_attn_packed(mi355x_ctx * ctx, const mi355x_attn_packed_des
         if ((type != MI355X_TYPE_F16 && type != MI355X_TYPE_BF16) || (d->k.ne[0] != 64 && d->k.ne[0] != 128) || Hkv < 1 || Hkv > 32768) return kv_refuse("attn_packed: k and v are F16 or BF16, [64 or 128, n_head_kv, rows]");
         if (!kv_rows_ok(&d->k, dim, Hkv) || !kv_rows_ok(&d->v, dim, Hkv) || d->v.type != type || d->v.ne[2] != d->k.ne[2]) return kv_refuse("attn_packed: v has another shape or type than k, or they are misaligned");
         if (d->k.nb[1] != d->v.nb[1] || d->k.nb[2] != d->v.nb[2]) return kv_refuse("attn_packed: k and v have other strides");
+        if (d->k.nb[1] < 0 || d->k.nb[2] < 0 || d->k.nb[2] > UINT32_MAX) return kv_refuse("attn_packed: k's strides");
         a.c.k = (char *) d->k.data; a.c.v = (char *) d->v.data; a.c.nb_head = d->k.nb[1]; a.c.nb_key = d->k.nb[2];
         a.rows_k = (int) d->k.ne[2];
     }

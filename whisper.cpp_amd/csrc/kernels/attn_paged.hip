@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     auto h_of = [&](int r) { return PACKED ? r - r / a.hg * a.hg : r; };
     const bool here = nl < rows && g0 + h_of(nl) < a.G;
     const int ql = min(q_of(nl), nq - 1);
+    auto v_row = [&](uint32_t put, int r) { return (LDS u32x4_t *) (size_t) ((put ^ (D == 128 ? (r & 1) << 7 : 0)) + r * RPL * (D * 2)); };
     bool bad = false;
     for (;;) {                                           // the parts of queries in this run
     const int seq = PACKED ? sp.s : a.seq ? a.seq[i] : i, held = PACKED ? 0 : held_of(a, seq);
@@ -181,9 +182,9 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
         return SRC == ROWS ? 0 : min(max(pg, 0), a.c.n_pages - 1);
     };
     auto place = [&](int t, int key, int pg) -> int64_t {
-        if (SRC == ROWS) return (int64_t) (k0 + key) * a.c.nb_key;
+        if (SRC == ROWS) return (int64_t) ((uint64_t) (uint32_t) (k0 + key) * (uint32_t) a.c.nb_key);
         const int p = SRC == BIG_PAGES ? __builtin_amdgcn_readfirstlane(pg) : __shfl(pg, key - t * TILE, 64);
-        return p * a.c.nb_page + (key & a.c.mask) * a.c.nb_key;
+        return (int64_t) ((uint64_t) (uint32_t) p * (uint32_t) a.c.nb_page + (uint64_t) (uint32_t) (key & a.c.mask) * (uint32_t) a.c.nb_key);
     };
     vec8 kr[2][KK]; u32x4_t vr[NV];
     auto fetch_k = [&](int t, int pg) {
@@ -235,15 +236,17 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
                 for (int r = 0; r < NV; r++) nf |= not_finite8<O>(vr[r]);
                 odd = __any(nf != 0);
             }
-            auto put_v = [&](int what) {                             // 0: as it is, 1: without what is not finite, 2: what that was
+            if (PACKED && odd) {
                 #pragma unroll
                 for (int r = 0; r < NV; r++) {
                     u32x4_t x = vr[r], kind = { 0, 0, 0, 0 };
-                    if (what) take_apart<O>(x, kind);
-                    *(LDS u32x4_t *) (size_t) ((put ^ (D == 128 ? (r & 1) << 7 : 0)) + r * RPL * (D * 2)) = what == 2 ? kind : x;
+                    take_apart<O>(x, kind);
+                    *v_row(put, r) = x;
                 }
-            };
-            if (PACKED && odd) put_v(1); else put_v(0);
+            } else {
+                #pragma unroll
+                for (int r = 0; r < NV; r++) *v_row(put, r) = vr[r];
+            }
             if (more && !odd) {
                 fetch_v(t + waves, pg);
                 pg = ask_pages(t + 2 * waves);
@@ -290,7 +293,12 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
                 for (int n = NT - 1; n >= 0; n--) o[d] = O::mfma16(vf, pf[n], o[d]);
             }
             if (PACKED && odd) {
-                put_v(2);
+                #pragma unroll
+                for (int r = 0; r < NV; r++) {
+                    u32x4_t x = vr[r], kind = { 0, 0, 0, 0 };
+                    take_apart<O>(x, kind);
+                    *v_row(put, r) = kind;
+                }
                 vec8 seen;
                 #pragma unroll
                 for (int e = 0; e < 8; e++) {

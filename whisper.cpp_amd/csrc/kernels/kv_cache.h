@@ -36,6 +36,7 @@ static inline int kv_view(const mi355x_kv_cache * c, kvc * o) {
     if (((uintptr_t) c->table | (uintptr_t) c->len | (uintptr_t) c->ref | (uintptr_t) c->status | (uintptr_t) c->work) % 4) return kv_refuse("kv cache: misaligned tables");
     const int64_t row = c->head_dim * 2;
     if (c->nb_key < row || c->nb_head < row || c->nb_page < row) return kv_refuse("kv cache: strides smaller than a row");
+    if (c->nb_key > UINT32_MAX || c->nb_page > UINT32_MAX) return kv_refuse("kv cache: strides of 4 GiB and more");
     o->k = (char *) c->k; o->v = (char *) c->v; o->nb_key = c->nb_key; o->nb_head = c->nb_head; o->nb_page = c->nb_page;
     o->table = c->table; o->len = c->len; o->ref = c->ref; o->status = c->status; o->work = (int *) c->work;
     o->n_pages = c->n_pages; o->n_seq = c->n_seq; o->max_pages = c->max_pages;

@@ -76,8 +76,12 @@ struct KvAppendArgs {
 __device__ __forceinline__ bool kv_reserve(const KvAppendArgs & a, const kv_work & w, uint32_t * seen, int * part, int * shared) {
     const int tid = threadIdx.x, cap = a.c.max_pages << a.c.shift;
     const int words = (a.c.n_seq + 31) >> 5;
+    // the counts of the lowest pages are asked for first: what the entries need is known several loads later
+    int low[4];
+    #pragma unroll
+    for (int e = 0; e < 4; e++) low[e] = tid * 4 + e < a.c.n_pages ? a.c.ref[tid * 4 + e] : 1;
     for (int i = tid; i < words; i += KV_WG) seen[i] = 0;
-    if (tid == 0) shared[0] = 0;
+    if (tid == 0) shared[0] = shared[1] = 0;
     __syncthreads();
     int need_all = 0, bad = 0;
     for (int base = 0; base < a.n; base += KV_WG) {
@@ -103,6 +107,7 @@ __device__ __forceinline__ bool kv_reserve(const KvAppendArgs & a, const kv_work
                 }
             }
             w.start[i] = start; w.copied[i] = copied;
+            if (copied >= 0) shared[1] = 1;                          // some entry copies its last page
         }
         int total;
         const int at = wg_scan(need, part, total);
@@ -119,7 +124,7 @@ __device__ __forceinline__ bool kv_reserve(const KvAppendArgs & a, const kv_work
             const int p0 = base + tid * 4;
             int fr[4], cnt = 0;
             #pragma unroll
-            for (int e = 0; e < 4; e++) { fr[e] = p0 + e < a.c.n_pages && a.c.ref[p0 + e] == 0; cnt += fr[e]; }
+            for (int e = 0; e < 4; e++) { fr[e] = p0 + e < a.c.n_pages && (base ? a.c.ref[p0 + e] : low[e]) == 0; cnt += fr[e]; }
             int total, at = wg_scan(cnt, part, total) + found;
             #pragma unroll
             for (int e = 0; e < 4; e++) if (fr[e]) { if (at < need_all) w.pages[at] = p0 + e; at++; }
@@ -145,25 +150,47 @@ __device__ __forceinline__ bool kv_reserve(const KvAppendArgs & a, const kv_work
     return true;
 }
 
-// one 16-byte piece of a row into its place, rounded to the cache's type
-__device__ __forceinline__ void kv_put(const KvAppendArgs & a, int row, int piece, int64_t at) {
-    const bool isv = piece >= a.nch;
-    const int q = isv ? piece - a.nch : piece, head = q >> a.cshift, ch = q & ((1 << a.cshift) - 1);
-    const char * src = isv ? a.v + row * a.v_nb2 + head * a.v_nb1 : a.k + row * a.k_nb2 + head * a.k_nb1;
-    char * dst = (isv ? a.c.v : a.c.k) + at + head * a.c.nb_head + ch * 16;
-    if (a.type_in == (a.bf16 ? MI355X_TYPE_BF16 : MI355X_TYPE_F16)) { *(uint4 *) dst = *(const uint4 *) (src + ch * 16); return; }
-    float f[8];
-    load8(src + (int64_t) ch * (a.type_in == MI355X_TYPE_F32 ? 32 : 16), a.type_in, f);
-    if (a.bf16) {
-        bf16x8_t o;
+// `count` pieces of 16 bytes (as stored) of rows r0 .. into their places at[], by NT threads, rounded to the cache's type: four loads of a thread before
+// its stores, which might be to the same memory as far as the compiler knows
+template <int NT> __device__ __forceinline__ void kv_put(const KvAppendArgs & a, int r0, const int64_t * at, int count) {
+    const int per = 2 * a.nch;
+    const bool same = a.type_in == (a.bf16 ? MI355X_TYPE_BF16 : MI355X_TYPE_F16);
+    for (int j0 = threadIdx.x; j0 < count; j0 += 4 * NT) {
+        char * dst[4]; const char * src[4];
         #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = (__bf16) f[e];
-        *(bf16x8_t *) dst = o;
-    } else {
-        half8_t o;
+        for (int u = 0; u < 4; u++) {
+            const int j = min(j0 + u * NT, count - 1), r = (int) __umulhi((uint32_t) j, a.div_m);     // j / per: exact, j * per < 2^32
+            const int piece = j - r * per;
+            const bool isv = piece >= a.nch;
+            const int q = isv ? piece - a.nch : piece, head = q >> a.cshift, ch = q & ((1 << a.cshift) - 1);
+            src[u] = (isv ? a.v + (r0 + r) * a.v_nb2 + head * a.v_nb1 : a.k + (r0 + r) * a.k_nb2 + head * a.k_nb1) + ch * (a.type_in == MI355X_TYPE_F32 ? 32 : 16);
+            dst[u] = j0 + u * NT < count && at[r] >= 0 ? (isv ? a.c.v : a.c.k) + at[r] + head * a.c.nb_head + ch * 16 : nullptr;
+        }
+        u32x4_t x[4];
+        if (same) {
+            #pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = *(const u32x4_t *) src[u];
+        } else {
+            float f[4][8];
+            #pragma unroll
+            for (int u = 0; u < 4; u++) load8(src[u], a.type_in, f[u]);
+            #pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (a.bf16) {
+                    bf16x8_t o;
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) o[e] = (__bf16) f[u][e];
+                    __builtin_memcpy(&x[u], &o, 16);
+                } else {
+                    half8_t o;
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) o[e] = (half_t) f[u][e];
+                    __builtin_memcpy(&x[u], &o, 16);
+                }
+            }
+        }
         #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = (half_t) f[e];
-        *(half8_t *) dst = o;
+        for (int u = 0; u < 4; u++) if (dst[u]) *(u32x4_t *) dst[u] = x[u];
     }
 }
 
@@ -179,13 +206,13 @@ __device__ __forceinline__ int64_t kv_place(const KvAppendArgs & a, const kv_wor
 }
 
 // the rows of entry i's last page that its sequence shared, into the page of its own
-template <int NT> __device__ __forceinline__ void kv_copy_shared(const KvAppendArgs & a, const kv_work & w, int i) {
+template <int NT> __device__ __forceinline__ void kv_copy_shared(const KvAppendArgs & a, const kv_work & w, int i, int tid) {
     const int p = w.copied[i];
     if (p < 0) return;
     const int keys = w.start[i] & a.c.mask, to = a.c.table[(int64_t) a.seq[i] * a.c.max_pages + (w.start[i] >> a.c.shift)];
     if (to < 0 || to >= a.c.n_pages) return;
     const int per = keys << a.cshift;                                // pieces of one head
-    for (int j = threadIdx.x; j < 2 * a.c.Hkv * per; j += NT) {
+    for (int j = tid; j < 2 * a.c.Hkv * per; j += NT) {
         const int hv = j / per, q = j - hv * per, head = hv >> 1;
         const int64_t at = head * a.c.nb_head + (q >> a.cshift) * a.c.nb_key + (q & ((1 << a.cshift) - 1)) * 16;
         char * pool = hv & 1 ? a.c.v : a.c.k;
@@ -195,7 +222,7 @@ template <int NT> __device__ __forceinline__ void kv_copy_shared(const KvAppendA
 
 __global__ void __launch_bounds__(KV_WG) k_kv_reserve(const KvAppendArgs a) {
     extern __shared__ uint32_t seen[];
-    __shared__ int part[KV_WG / 64], shared[1];
+    __shared__ int part[KV_WG / 64], shared[2];
     kv_reserve(a, kv_work_of(a.c.work, a.c.n_seq, a.c.n_pages), seen, part, shared);
 }
 
@@ -205,16 +232,29 @@ __global__ void __launch_bounds__(KV_WG) k_kv_reserve(const KvAppendArgs a) {
 __global__ void __launch_bounds__(256) k_kv_write(const KvAppendArgs a) {
     const kv_work w = kv_work_of(a.c.work, a.c.n_seq, a.c.n_pages);
     if (w.flag[0] == 0) return;
-    if ((int) blockIdx.x >= a.row_blocks) { kv_copy_shared<256>(a, w, blockIdx.x - a.row_blocks); return; }
+    if ((int) blockIdx.x >= a.row_blocks) { kv_copy_shared<256>(a, w, blockIdx.x - a.row_blocks, threadIdx.x); return; }
     __shared__ int64_t at[KV_RB];
     const int r0 = blockIdx.x * a.rb, nr = min(a.rb, a.rows - r0);
     if ((int) threadIdx.x < nr) at[threadIdx.x] = kv_place(a, w, r0 + threadIdx.x);
     __syncthreads();
-    const int per = 2 * a.nch;
-    for (int j = threadIdx.x; j < nr * per; j += 256) {
-        const int r = (int) __umulhi((uint32_t) j, a.div_m);         // j / per: exact, j < KV_RB * per and KV_RB * per^2 < 2^32
-        if (at[r] >= 0) kv_put(a, r0 + r, j - r * per, at[r]);
-    }
+    kv_put<256>(a, r0, at, nr * 2 * a.nch);
+}
+
+// few rows: pages and rows by one workgroup, without the second launch, as long as that is one batch of loads for each thread (with the
+// truncation before it, 20 heads of 64: one row 7.7 us, two launches 11.4; eight rows 11.9, 12.8).  One CU takes too long for more: 32 rows of 20 heads of 64 (10240 pieces) 14.9 us, where two launches take 5.7 + 4.6.
+#define KV_SMALL_ROWS 256
+#define KV_SMALL_PIECES (4 * KV_WG)
+__global__ void __launch_bounds__(KV_WG) k_kv_append_small(const KvAppendArgs a) {
+    extern __shared__ uint32_t seen[];
+    __shared__ int part[KV_WG / 64], shared[2];
+    __shared__ int64_t at[KV_SMALL_ROWS];
+    const kv_work w = kv_work_of(a.c.work, a.c.n_seq, a.c.n_pages);
+    if (!kv_reserve(a, w, seen, part, shared)) return;
+    __syncthreads();                                                 // table and lists as they are now
+    if ((int) threadIdx.x < a.rows) at[threadIdx.x] = kv_place(a, w, threadIdx.x);
+    if (shared[1]) for (int i = threadIdx.x >> 6; i < a.n; i += KV_WG / 64) kv_copy_shared<64>(a, w, i, threadIdx.x & 63);
+    __syncthreads();
+    kv_put<KV_WG>(a, 0, at, a.rows * 2 * a.nch);
 }
 
 extern "C" int mi355x_kv_append(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n, const int32_t * seq, const int32_t * cu, const mi355x_tensor * k, const mi355x_tensor * v) {
@@ -234,6 +274,8 @@ extern "C" int mi355x_kv_append(mi355x_ctx * ctx, const mi355x_kv_cache * c, int
     a.cshift = c->head_dim == 64 ? 3 : 4; a.nch = c->n_head_kv << a.cshift;
     a.div_m = (uint32_t) ((((uint64_t) 1 << 32) + 2 * a.nch - 1) / (2 * a.nch));
     const uint32_t lds = (uint32_t) ((c->n_seq + 31) / 32 * 4);
+    if (a.rows > 0 && a.rows <= KV_SMALL_ROWS && (int64_t) a.rows * 2 * a.nch <= KV_SMALL_PIECES)
+        return emit(ctx, "kv_append", k_kv_append_small, dim3(1), dim3(KV_WG), lds, a);
     int rc1 = emit(ctx, "kv_reserve", k_kv_reserve, dim3(1), dim3(KV_WG), lds, a);
     if (rc1 || a.rows == 0) return rc1;
     a.rb = a.rows >= 4096 ? KV_RB : 1;
