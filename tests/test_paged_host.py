@@ -85,6 +85,8 @@ def test_attention_of_one_token_refuses_what_it_cannot_do():
     refused("mi355x_attn_paged", C.byref(c), None)
     assert ka.attn_paged_work_bytes(c, 3, 2) > 64                    # 65536 keys: split, so the work area is wanted
     assert ka.attn_paged_work_bytes(c, 3, 2, 100) == 0               # at most 100: not
+    big = cache(max_pages=1 << 26)                                   # 2^30 keys: more than 31 of such queries are not split, their costs would not fit 32 bits
+    assert ka.attn_paged_work_bytes(big, 31, 2) > 0 and ka.attn_paged_work_bytes(big, 32, 2) == 0
     assert ka.attn_paged_work_bytes(c, 3, 3) == 0 and ka.attn_paged_work_bytes(c, 0, 2) == 0
     assert ka.kv_work_bytes(4, 8) > 0 and ka.kv_work_bytes(0, 8) == 0 and ka.kv_work_bytes(4, -1) == 0
 

@@ -423,7 +423,7 @@ struct paged_split { int W, rec_rows; size_t floats, bytes; };
 static paged_split paged_split_of(const mi355x_kv_cache * c, int64_t n, int64_t n_head, int max_len) {
     paged_split r = { 0, 0, 0, 0 };
     const int64_t cap = (int64_t) c->max_pages * c->page_size, len = max_len > 0 && max_len < cap ? max_len : cap, G = n_head / c->n_head_kv, units = c->n_head_kv * ((G + 15) / 16);
-    if (len <= 1024 || (n * units >= CHIP_RUNS && len * c->head_dim <= 131072) || n > 4096) return r;
+    if (len <= 1024 || (n * units >= CHIP_RUNS && len * c->head_dim <= 131072) || n > 4096 || n * (cap / TILE + 1 + OVERHEAD) > INT32_MAX / 2) return r;   // (the last: sums of costs are 32 bits)
     r.W = units < CHIP_RUNS ? (int) (CHIP_RUNS / units) : 1;
     r.rec_rows = (int) (G < 16 ? G : 16);
     r.floats = (size_t) units * (r.W + n) * r.rec_rows;
