@@ -150,49 +150,61 @@ __device__ __forceinline__ bool kv_reserve(const KvAppendArgs & a, const kv_work
     return true;
 }
 
-// `count` pieces of 16 bytes (as stored) of rows r0 .. into their places at[], by NT threads, rounded to the cache's type: four loads of a thread before
-// its stores, which might be to the same memory as far as the compiler knows
-template <int NT> __device__ __forceinline__ void kv_put(const KvAppendArgs & a, int r0, const int64_t * at, int count) {
-    const int per = 2 * a.nch;
-    const bool same = a.type_in == (a.bf16 ? MI355X_TYPE_BF16 : MI355X_TYPE_F16);
-    for (int j0 = threadIdx.x; j0 < count; j0 += 4 * NT) {
-        char * dst[4]; const char * src[4];
+// U pieces of 16 bytes (as stored) of each of NT threads, from j0 on, of the `count` pieces of rows r0 ..: first all loads, which do not wait for the rows'
+// places, then the stores to the places at[], rounded to the cache's type
+template <int NT, int U> struct kv_pieces {
+    u32x4_t x[U][2];
+    // piece j's row (j / per: exact, j * per < 2^32), V or K, head and piece of the head
+    static __device__ __forceinline__ void of(const KvAppendArgs & a, int j, int & r, bool & isv, int & head, int & ch) {
+        r = (int) __umulhi((uint32_t) j, a.div_m);
+        const int piece = j - r * 2 * a.nch;
+        isv = piece >= a.nch;
+        const int q = isv ? piece - a.nch : piece;
+        head = q >> a.cshift; ch = q & ((1 << a.cshift) - 1);
+    }
+    __device__ __forceinline__ void load(const KvAppendArgs & a, int r0, int count, int j0) {
+        const char * src[U];
         #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int j = min(j0 + u * NT, count - 1), r = (int) __umulhi((uint32_t) j, a.div_m);     // j / per: exact, j * per < 2^32
-            const int piece = j - r * per;
-            const bool isv = piece >= a.nch;
-            const int q = isv ? piece - a.nch : piece, head = q >> a.cshift, ch = q & ((1 << a.cshift) - 1);
+        for (int u = 0; u < U; u++) {
+            int r, head, ch; bool isv;
+            of(a, min(j0 + u * NT, count - 1), r, isv, head, ch);
             src[u] = (isv ? a.v + (r0 + r) * a.v_nb2 + head * a.v_nb1 : a.k + (r0 + r) * a.k_nb2 + head * a.k_nb1) + ch * (a.type_in == MI355X_TYPE_F32 ? 32 : 16);
-            dst[u] = j0 + u * NT < count && at[r] >= 0 ? (isv ? a.c.v : a.c.k) + at[r] + head * a.c.nb_head + ch * 16 : nullptr;
         }
-        u32x4_t x[4];
-        if (same) {
+        #pragma unroll
+        for (int u = 0; u < U; u++) x[u][0] = *(const u32x4_t *) src[u];
+        if (a.type_in == MI355X_TYPE_F32) {
             #pragma unroll
-            for (int u = 0; u < 4; u++) x[u] = *(const u32x4_t *) src[u];
-        } else {
-            float f[4][8];
-            #pragma unroll
-            for (int u = 0; u < 4; u++) load8(src[u], a.type_in, f[u]);
-            #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < U; u++) x[u][1] = ((const u32x4_t *) src[u])[1];
+        }
+    }
+    __device__ __forceinline__ void store(const KvAppendArgs & a, const int64_t * at, int count, int j0) {
+        const bool same = a.type_in == (a.bf16 ? MI355X_TYPE_BF16 : MI355X_TYPE_F16);
+        #pragma unroll
+        for (int u = 0; u < U; u++) {
+            int r, head, ch; bool isv;
+            of(a, min(j0 + u * NT, count - 1), r, isv, head, ch);
+            if (j0 + u * NT >= count || at[r] < 0) continue;
+            u32x4_t y = x[u][0];
+            if (!same) {
+                char raw[32]; float f[8];
+                __builtin_memcpy(raw, &x[u][0], 16); __builtin_memcpy(raw + 16, &x[u][1], 16);
+                load8(raw, a.type_in, f);
                 if (a.bf16) {
                     bf16x8_t o;
                     #pragma unroll
-                    for (int e = 0; e < 8; e++) o[e] = (__bf16) f[u][e];
-                    __builtin_memcpy(&x[u], &o, 16);
+                    for (int e = 0; e < 8; e++) o[e] = (__bf16) f[e];
+                    __builtin_memcpy(&y, &o, 16);
                 } else {
                     half8_t o;
                     #pragma unroll
-                    for (int e = 0; e < 8; e++) o[e] = (half_t) f[u][e];
-                    __builtin_memcpy(&x[u], &o, 16);
+                    for (int e = 0; e < 8; e++) o[e] = (half_t) f[e];
+                    __builtin_memcpy(&y, &o, 16);
                 }
             }
+            *(u32x4_t *) ((isv ? a.c.v : a.c.k) + at[r] + head * a.c.nb_head + ch * 16) = y;
         }
-        #pragma unroll
-        for (int u = 0; u < 4; u++) if (dst[u]) *(u32x4_t *) dst[u] = x[u];
     }
-}
+};
 
 // byte offset of packed row r's place in the pools, -1 if the row belongs to no sequence
 __device__ __forceinline__ int64_t kv_place(const KvAppendArgs & a, const kv_work & w, int r) {
@@ -226,18 +238,23 @@ __global__ void __launch_bounds__(KV_WG) k_kv_reserve(const KvAppendArgs a) {
     kv_reserve(a, kv_work_of(a.c.work, a.c.n_seq, a.c.n_pages), seen, part, shared);
 }
 
-// rows into their pages: rb rows per workgroup, whose places are looked up once; behind them one workgroup per entry for shared last pages.
-// Bound by HBM (rows in, rows out).
-#define KV_RB 8
+// rows into their pages: rb rows per workgroup, whose places are looked up while the rows are on their way; behind them one workgroup per entry for shared
+// last pages.  Bound by HBM (rows in, rows out) once there are enough rows: with the two launches before it (9 us) 17321 rows of 8 heads of 128, 142 MB in
+// and out, 44 us; four pieces of a thread at a time (eight: 46; places first, then the rows: 45, and 300 rows a sequence 15.1 instead of 14.0).
+#define KV_U 4
+#define KV_RB 16
 __global__ void __launch_bounds__(256) k_kv_write(const KvAppendArgs a) {
     const kv_work w = kv_work_of(a.c.work, a.c.n_seq, a.c.n_pages);
-    if (w.flag[0] == 0) return;
-    if ((int) blockIdx.x >= a.row_blocks) { kv_copy_shared<256>(a, w, blockIdx.x - a.row_blocks, threadIdx.x); return; }
+    if ((int) blockIdx.x >= a.row_blocks) { if (w.flag[0]) kv_copy_shared<256>(a, w, blockIdx.x - a.row_blocks, threadIdx.x); return; }
     __shared__ int64_t at[KV_RB];
-    const int r0 = blockIdx.x * a.rb, nr = min(a.rb, a.rows - r0);
+    const int r0 = blockIdx.x * a.rb, nr = min(a.rb, a.rows - r0), count = nr * 2 * a.nch;
+    kv_pieces<256, KV_U> p;
+    p.load(a, r0, count, threadIdx.x);
+    if (w.flag[0] == 0) return;
     if ((int) threadIdx.x < nr) at[threadIdx.x] = kv_place(a, w, r0 + threadIdx.x);
     __syncthreads();
-    kv_put<256>(a, r0, at, nr * 2 * a.nch);
+    p.store(a, at, count, threadIdx.x);
+    for (int j0 = threadIdx.x + KV_U * 256; j0 < count; j0 += KV_U * 256) { p.load(a, r0, count, j0); p.store(a, at, count, j0); }
 }
 
 // few rows: pages and rows by one workgroup, without the second launch, as long as that is one batch of loads for each thread (with the
@@ -249,12 +266,15 @@ __global__ void __launch_bounds__(KV_WG) k_kv_append_small(const KvAppendArgs a)
     __shared__ int part[KV_WG / 64], shared[2];
     __shared__ int64_t at[KV_SMALL_ROWS];
     const kv_work w = kv_work_of(a.c.work, a.c.n_seq, a.c.n_pages);
+    const int count = a.rows * 2 * a.nch;
+    kv_pieces<KV_WG, KV_SMALL_PIECES / KV_WG> p;
+    p.load(a, 0, count, threadIdx.x);
     if (!kv_reserve(a, w, seen, part, shared)) return;
     __syncthreads();                                                 // table and lists as they are now
     if ((int) threadIdx.x < a.rows) at[threadIdx.x] = kv_place(a, w, threadIdx.x);
     if (shared[1]) for (int i = threadIdx.x >> 6; i < a.n; i += KV_WG / 64) kv_copy_shared<64>(a, w, i, threadIdx.x & 63);
     __syncthreads();
-    kv_put<KV_WG>(a, 0, at, a.rows * 2 * a.nch);
+    p.store(a, at, count, threadIdx.x);
 }
 
 extern "C" int mi355x_kv_append(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n, const int32_t * seq, const int32_t * cu, const mi355x_tensor * k, const mi355x_tensor * v) {
@@ -278,7 +298,8 @@ extern "C" int mi355x_kv_append(mi355x_ctx * ctx, const mi355x_kv_cache * c, int
         return emit(ctx, "kv_append", k_kv_append_small, dim3(1), dim3(KV_WG), lds, a);
     int rc1 = emit(ctx, "kv_reserve", k_kv_reserve, dim3(1), dim3(KV_WG), lds, a);
     if (rc1 || a.rows == 0) return rc1;
-    a.rb = a.rows >= 4096 ? KV_RB : 1;
+    a.rb = 1;
+    if (a.rows >= 4096) { a.rb = KV_U * 256 / (2 * a.nch); a.rb = a.rb < 1 ? 1 : a.rb > KV_RB ? KV_RB : a.rb; }
     a.row_blocks = (a.rows + a.rb - 1) / a.rb;
     const double bytes = (double) a.rows * a.nch * 2 * (16 + (k->type == MI355X_TYPE_F32 ? 32 : 16));
     return emit(ctx, "kv_write", k_kv_write, dim3((uint32_t) (a.row_blocks + n)), dim3(256), 0, a, bytes);
