@@ -458,6 +458,32 @@ def test_infinities_and_nan_reach_only_the_rows_that_see_them(gpu, kind, page, m
     packed_case(gpu, kind, kind, kind, 64, 2, 2, q, ks, page=page, max_q=max_q, window=2, spoil={(0, late - 2): (nan, nan), (1, ks[1] - 4): (1.0, -inf)})
 
 
+@pytest.mark.parametrize("kind,dim,page", [("f16", 64, 16), ("bf16", 128, 64)])
+@pytest.mark.parametrize("keys,window", [(75, 0), (75, 20), (1501, 0), (1501, 1100)])
+def test_infinities_in_the_first_and_last_key_of_one_token_stay_what_they_are(gpu, kind, dim, page, keys, window):
+    """keys outside the span stand for none of its values, at both ends of a tile"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=1, n_pages=-(-keys // page), max_pages=-(-keys // page), page=page, heads=2, dim=dim, kind=kind)
+    assert p.append([(0, keys)], kind) == 0
+    q = torch.randn(1, 4, dim, generator=p.gen, device="cuda").to(dt(torch, kind))
+    work = torch.empty(max(16, ka.attn_paged_work_bytes(p.c, 1, 4, 0)), dtype=torch.uint8, device="cuda")
+    clean, out = torch.empty(1, 4, dim, device="cuda"), torch.empty(1, 4, dim, device="cuda")
+    p.run(ctx.attn_paged_call(p.c, q, clean, scale=dim ** -0.5, window=window, work=work))
+    first, last = keys - window if window else 0, keys - 1
+    for key, d, x in ((last, 3, float("inf")), (last, 4, float("-inf")), (first, 5, float("inf")), (first, 6, float("-inf"))):
+        p.v[p.rows[0][key // page], :, key % page, d] = x
+    p.run(ctx.attn_paged_call(p.c, q, out, scale=dim ** -0.5, window=window, work=work))
+    assert out[..., [3, 5]].isposinf().all() and out[..., [4, 6]].isneginf().all()
+    clean[..., 3:7] = out[..., 3:7] = 0.0
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("page,max_q,ks", [(0, 0, [3, 40]), (16, 0, [3, 40]), (0, 8, [3, 600]), (16, 8, [3, 600])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_window_beyond_every_length_is_none(gpu, page, max_q, ks, causal):
+    packed_case(gpu, "f16", "f16", "f16", 64, 1, 2, [8, 8], ks, page=page, max_q=max_q, causal=causal, window=2**31 - 1)
+
+
 def test_the_largest_and_smallest_values_of_the_type(gpu):
     """keys and values at the type's ends: scores of +-6e4 * |q| * scale do not overflow F32, one weight takes it all"""
     ctx, ka, torch = gpu

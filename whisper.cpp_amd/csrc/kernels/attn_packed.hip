@@ -415,6 +415,7 @@ extern "C" int mi355x_attn_packed(mi355x_ctx * ctx, const mi355x_attn_packed_des
     a.c2 = fmaxf(fabsf(d->scale) * 1.4426950408889634f, 1e-37f); a.flip = d->scale < 0.0f; a.n = d->n; a.rows_q = (int) rows; a.causal = d->causal != 0; a.window = d->window;
     a.G = (int) (H / Hkv); a.Hkv = (int) Hkv;
     const bool f16 = type == MI355X_TYPE_F16, paged = d->cache != nullptr;
+    if (paged ? a.window >= (int64_t) d->cache->max_pages * d->cache->page_size : a.window >= a.rows_k) a.window = 0;      // no key lies before it
     const int64_t keys = paged ? (int64_t) d->cache->max_pages * d->cache->page_size : a.rows_k / d->n;       // of a sequence, as far as the host knows
     if (dim == 64) return f16 ? (paged ? launch_packed<f16_ops, 64, true>(ctx, a, Hkv, d->max_q, keys) : launch_packed<f16_ops, 64, false>(ctx, a, Hkv, d->max_q, keys))
                               : (paged ? launch_packed<bf16_ops, 64, true>(ctx, a, Hkv, d->max_q, keys) : launch_packed<bf16_ops, 64, false>(ctx, a, Hkv, d->max_q, keys));

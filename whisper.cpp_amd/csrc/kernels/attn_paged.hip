@@ -244,6 +244,13 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
                     *v_row(put, r) = x;
                 }
             } else {
+                if (!PACKED && (t * TILE < sp.lo || t * TILE + TILE > sp.hi)) {                      // rows that stand for none: their weight is zero, which an infinity would not obey
+                    #pragma unroll
+                    for (int r = 0; r < NV; r++) {
+                        const int key = t * TILE + r * RPL + wkey;
+                        if (key < sp.lo || key >= sp.hi) vr[r] = u32x4_t{ 0, 0, 0, 0 };
+                    }
+                }
                 #pragma unroll
                 for (int r = 0; r < NV; r++) *v_row(put, r) = vr[r];
             }
