@@ -8,12 +8,11 @@
 //                  S^T = K.Q^T and O^T = V^T.P^T on v_mfma_f32_32x32x16: a lane owns one row, so maximum, sum and rescaling are the lane's own scalars,
 //                  and P goes from registers to the second product.  K and V rows lie in LDS as they come, 16-byte pieces permuted so that neither the
 //                  row reads (K) nor the transposing reads (V) meet in a bank.  The two waves of a SIMD run half a step apart, one in the matrix products
-//                  (PV of the tile before, QK of this one) while the other is in the softmax: 8192 rows, 32 / 8 heads of 128, BF16: 595 us = 923
+//                  (PV of the tile before, QK of this one) while the other is in the softmax: 8192 rows, 32 / 8 heads of 128, BF16: 546 us = 1007
 //                  TFLOP/s (both waves in step, and LDS rows at 8-byte addresses: 1555 us).
 // A masked weight is an exact zero, but zero times an infinity or a NaN is none: where a tile that is masked in part holds such values, they are taken
 // out on the way into LDS and counted over the keys that a row sees, so that a row never meets what it does not see.
 #include "kv_cache.h"
-
 
 // what a 16-byte piece's number in its row is changed by (exclusive-or): the rows that an instruction reads together lie in different banks
 template <int D> __device__ __forceinline__ int k_swap(int key) { return D == 128 ? key & 15 : key >> 1 & 7; }
@@ -25,7 +24,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
     typedef typename O::elem elem;
     constexpr int KK = D / 16, NI = D / 32;
     constexpr int PCS = D / 8;                                        // 16-byte pieces of a row
-    constexpr int KT = NW == 8 || KG == 2 ? 64 : 32;                             // keys of a tile
+    constexpr int KT = NW == 8 || KG == 2 ? 64 : 32;                     // keys of a tile
     constexpr int KA = NW == 8 ? 2 : 1, VA = KA - 1;                  // tiles that K and V are in LDS ahead of the step that they are written in
     constexpr int SLOTS = NW == 8 ? 3 : 1;                            // in use at a time: K tiles t .. t+2, V tiles t-1 .. t+1 (one of each where all waves are in step)
     constexpr int NL = KT * PCS / (64 * NW), RPL = 64 * NW / PCS;               // pieces per thread and tile, K and V each; keys that lie between them
@@ -370,7 +369,7 @@ static int launch_packed_as(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv) {
 //       a second round of workgroups of equal length (4 x 512 + 2048 of a window, 32/8: 133; 96)
 template <typename O, int D, bool PAGED>
 static int launch_packed(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv, int max_q, int64_t keys) {
-    const int64_t rows = (int64_t) a.rows_q * a.G, per = (rows + a.n - 1) / a.n;     // rows (query x head of a group), and of one sequence on the average
+    const int64_t rows = (int64_t) a.rows_q * a.G;                   // query x head of a group
     const int64_t few = (int64_t) a.n * Hkv * ((max_q * (int64_t) a.G + 15) / 16);   // workgroups of 16 rows
     if (max_q > 0 && (int64_t) max_q * a.G <= 256 && few <= ctx->n_cu && keys >= 256) return mi355x_attn_few_rows(ctx, a, __is_same(O, f16_ops) ? MI355X_TYPE_F16 : MI355X_TYPE_BF16, D, PAGED);
     const int64_t wide = rows * Hkv / 256;                           // workgroups of 256 rows, if all were full
@@ -378,6 +377,7 @@ static int launch_packed(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv, int max_
         if (wide < 512 && keys >= 128) return launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv);
         return launch_packed_as<O, D, PAGED, 4, 1>(ctx, a, Hkv);
     } else {
+        const int64_t per = (rows + a.n - 1) / a.n;                  // of one sequence on the average
         const bool wedge = a.causal && a.window == 0 && keys <= 2 * (a.rows_q / a.n);
         if (wide <= (wedge ? ctx->n_cu : ctx->n_cu / 2) && keys >= 256) return per <= 64 ? launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv) : launch_packed_as<O, D, PAGED, 8, 2>(ctx, a, Hkv);
         return keys <= 768 ? launch_packed_as<O, D, PAGED, 4, 1>(ctx, a, Hkv) : launch_packed_as<O, D, PAGED, 8, 1>(ctx, a, Hkv);

@@ -79,7 +79,7 @@ __device__ __forceinline__ bool kv_reserve(const KvAppendArgs & a, const kv_work
     // the counts of the lowest pages are asked for first: what the entries need is known several loads later
     int low[4];
     #pragma unroll
-    for (int e = 0; e < 4; e++) low[e] = tid * 4 + e < a.c.n_pages ? a.c.ref[tid * 4 + e] : 1;
+    for (int e = 0; e < 4; e++) low[e] = a.c.ref[min(tid * 4 + e, a.c.n_pages - 1)];
     for (int i = tid; i < words; i += KV_WG) seen[i] = 0;
     if (tid == 0) shared[0] = shared[1] = 0;
     __syncthreads();
@@ -124,7 +124,9 @@ __device__ __forceinline__ bool kv_reserve(const KvAppendArgs & a, const kv_work
             const int p0 = base + tid * 4;
             int fr[4], cnt = 0;
             #pragma unroll
-            for (int e = 0; e < 4; e++) { fr[e] = p0 + e < a.c.n_pages && (base ? a.c.ref[p0 + e] : low[e]) == 0; cnt += fr[e]; }
+            for (int e = 0; e < 4; e++) if (base) low[e] = a.c.ref[min(p0 + e, a.c.n_pages - 1)];
+            #pragma unroll
+            for (int e = 0; e < 4; e++) { fr[e] = p0 + e < a.c.n_pages && low[e] == 0; cnt += fr[e]; }
             int total, at = wg_scan(cnt, part, total) + found;
             #pragma unroll
             for (int e = 0; e < 4; e++) if (fr[e]) { if (at < need_all) w.pages[at] = p0 + e; at++; }
@@ -403,7 +405,9 @@ __global__ void __launch_bounds__(KV_WG) k_kv_rank(const KvCompactArgs a) {
         const int p0 = base + threadIdx.x * 4;
         int held[4], cnt = 0;
         #pragma unroll
-        for (int e = 0; e < 4; e++) { held[e] = p0 + e < a.a.n_pages && a.a.ref[p0 + e] > 0; cnt += held[e]; }
+        for (int e = 0; e < 4; e++) held[e] = a.a.ref[min(p0 + e, a.a.n_pages - 1)];
+        #pragma unroll
+        for (int e = 0; e < 4; e++) { held[e] = p0 + e < a.a.n_pages && held[e] > 0; cnt += held[e]; }
         int total, at = wg_scan(cnt, part, total) + used;
         #pragma unroll
         for (int e = 0; e < 4; e++) if (p0 + e < a.a.n_pages) { w.rank[p0 + e] = held[e] ? at : -1; if (held[e]) w.pages[at++] = p0 + e; }
@@ -435,24 +439,19 @@ __global__ void __launch_bounds__(256) k_kv_compact(const KvCompactArgs a) {
     if (r >= used) return;
     const int64_t from = w.pages[r] * a.a.nb_page, to = r * a.b.nb_page;
     const int per = a.a.Hkv << (a.a.shift + a.cshift);               // pieces of a page in one pool
-    uint4 x[KV_SLICE / 256];
-    int64_t at[KV_SLICE / 256];
+    // every load before the first store, and none under a condition: one that might not happen is not asked for before its store
+    u32x4_t x[KV_SLICE / 256];
+    char * dst[KV_SLICE / 256];
     #pragma unroll
     for (int e = 0; e < KV_SLICE / 256; e++) {
-        const int j0 = slice * KV_SLICE + e * 256 + threadIdx.x;
-        const bool isv = j0 >= per;
-        const int j = isv ? j0 - per : j0;
-        at[e] = -1;
-        if (j >= per) continue;
-        const int ch = j & ((1 << a.cshift) - 1), row = j >> a.cshift, key = row & a.a.mask, head = row >> a.a.shift;
-        x[e] = *(const uint4 *) ((isv ? a.a.v : a.a.k) + from + head * a.a.nb_head + key * a.a.nb_key + ch * 16);
-        at[e] = to + head * a.b.nb_head + key * a.b.nb_key + ch * 16;
+        const int j0 = slice * KV_SLICE + e * 256 + threadIdx.x, j1 = min(j0, 2 * per - 1);
+        const bool isv = j1 >= per;
+        const int j = isv ? j1 - per : j1, ch = j & ((1 << a.cshift) - 1), row = j >> a.cshift, key = row & a.a.mask, head = row >> a.a.shift;
+        x[e] = *(const u32x4_t *) ((isv ? a.a.v : a.a.k) + from + head * a.a.nb_head + key * a.a.nb_key + ch * 16);
+        dst[e] = j0 < 2 * per ? (isv ? a.b.v : a.b.k) + to + head * a.b.nb_head + key * a.b.nb_key + ch * 16 : nullptr;
     }
     #pragma unroll
-    for (int e = 0; e < KV_SLICE / 256; e++) {
-        const int j0 = slice * KV_SLICE + e * 256 + threadIdx.x;
-        if (at[e] >= 0) *(uint4 *) ((j0 >= per ? a.b.v : a.b.k) + at[e]) = x[e];
-    }
+    for (int e = 0; e < KV_SLICE / 256; e++) if (dst[e]) *(u32x4_t *) dst[e] = x[e];
 }
 extern "C" int mi355x_kv_compact(mi355x_ctx * ctx, const mi355x_kv_cache * from, const mi355x_kv_cache * to) {
     KvCompactArgs a; int rc = kv_view(from, &a.a);
