@@ -9,7 +9,7 @@
 //                  and P goes from registers to the second product.  K and V rows lie in LDS as they come, 16-byte pieces permuted so that neither the
 //                  row reads (K) nor the transposing reads (V) meet in a bank.  The two waves of a SIMD run half a step apart, one in the matrix products
 //                  (PV of the tile before, QK of this one) while the other is in the softmax: 8192 rows, 32 / 8 heads of 128, BF16: 546 us = 1007
-//                  TFLOP/s (both waves in step, and LDS rows at 8-byte addresses: 1555 us).
+//                  TFLOP/s (585 on another card; both waves in step, and LDS rows at 8-byte addresses: 1555 us).
 // A masked weight is an exact zero, but zero times an infinity or a NaN is none: where a tile that is masked in part holds such values, they are taken
 // out on the way into LDS and counted over the keys that a row sees, so that a row never meets what it does not see.
 #include "kv_cache.h"

@@ -10,7 +10,7 @@
 //                  product is the same for both operands).  K goes from memory to registers as the operand lies (64 consecutive bytes of a key per
 //                  instruction and 4 lanes), V through an area of LDS that belongs to the wave, read back transposed: no barrier in the loop, and the
 //                  next tile's 8 or 16 KB are on their way while one is computed.  974 MB of BF16 keys: 175 us = 5.6 TB/s (a loop that only
-//                  reads reaches 6.2 on this card, a copy 4.9); 351 MB in 64 queries of 1 .. 8192 keys: 81 us.
+//                  reads reaches 6.2 on this card, a copy 4.9); 351 MB in 64 queries of 1 .. 8192 keys: 81 us (a run for each wave instead of each workgroup: 80 to 83).
 //   k_attn_join    joins the parts of one query and head where the keys were split.
 // The same kernel serves packed sequences of few rows (attn_packed.hip says when): a tile's 16 columns are then (query, head) pairs, each with its own
 // range of keys.
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const PagedArgs a) {
 // Whether and how the keys are split.  A workgroup takes a query's keys (of one K/V head) alone where there are at most 1024 of them (448 keys, 8 heads of
 // 64: 7.3 us, where a second launch alone is 4), or where every CU has two such workgroups and none reads more than half a megabyte (32 x 1500, 20 heads of
 // 64: 48.6 us; split 52.1.  64 x 1 .. 2048, 8 heads of 128, a megabyte: 33.4; split 26.5).  Beyond that the costs of all queries are cut into as many
-// equal runs as workgroups of four waves fit the chip at once (two to a CU: 174 registers): every CU has the same to do, however the lengths differ, and
+// equal runs as workgroups of four waves fit the chip at once (two to a CU: 178 to 243 registers at 128 dims): every CU has the same to do, however the lengths differ, and
 // no workgroup starts late (2 x 100001 .. 131072 keys, 8 heads of 128: 175 us; three to a CU, in two rounds: 191).
 #define CHIP_RUNS (2 * 256)
 struct paged_split { int W, rec_rows; size_t floats, bytes; };

@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(KV_WG) k_kv_reserve(const KvAppendArgs a) {
 
 // rows into their pages: rb rows per workgroup, whose places are looked up while the rows are on their way; behind them one workgroup per entry for shared
 // last pages.  Bound by HBM (rows in, rows out) once there are enough rows: with the two launches before it (9 us) 17321 rows of 8 heads of 128, 142 MB in
-// and out, 44 us; four pieces of a thread at a time (eight: 46; places first, then the rows: 45, and 300 rows a sequence 15.1 instead of 14.0).
+// and out, 44 us, of which this is 28.7 (4.9 TB/s); four pieces of a thread at a time (eight: 46; places first, then the rows: 45, and 300 rows a sequence
+// 15.1 instead of 13.7).
 #define KV_U 4
 #define KV_RB 16
 __global__ void __launch_bounds__(256) k_kv_write(const KvAppendArgs a) {
@@ -259,8 +260,9 @@ __global__ void __launch_bounds__(256) k_kv_write(const KvAppendArgs a) {
     for (int j0 = threadIdx.x + KV_U * 256; j0 < count; j0 += KV_U * 256) { p.load(a, r0, count, j0); p.store(a, at, count, j0); }
 }
 
-// few rows: pages and rows by one workgroup, without the second launch, as long as that is one batch of loads for each thread (with the
-// truncation before it, 20 heads of 64: one row 7.7 us, two launches 11.4; eight rows 11.9, 12.8).  One CU takes too long for more: 32 rows of 20 heads of 64 (10240 pieces) 14.9 us, where two launches take 5.7 + 4.6.
+// few rows: pages and rows by one workgroup, without the second launch, as long as that is one batch of loads for each thread (with the truncation before
+// it, 20 heads of 64: one row 7.9 us, two launches 11.6; eight rows 11.3, 12.2).  One CU takes too long for more: 32 rows of 20 heads of 64 (10240 pieces)
+// 14.9 us by itself, where two launches take 5.3 + 4.9.
 #define KV_SMALL_ROWS 256
 #define KV_SMALL_PIECES (4 * KV_WG)
 __global__ void __launch_bounds__(KV_WG) k_kv_append_small(const KvAppendArgs a) {
@@ -394,7 +396,8 @@ extern "C" int mi355x_kv_fork(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// compact: the held pages' ranks (one workgroup), then pages and table.  Bound by HBM: every held page is read and written once.
+// compact: the held pages' ranks (one workgroup, 5 us for 10000), then pages and table.  Bound by HBM: every held page is read and written once.  Half a
+// gigabyte in and out: 91 us = 5.0 TB/s; three megabytes 7 us.
 // ---------------------------------------------------------------------------------------------------------------
 struct KvCompactArgs { kvc a, b; int cshift, slices, table_blocks; };
 __global__ void __launch_bounds__(KV_WG) k_kv_rank(const KvCompactArgs a) {
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(256) k_kv_compact(const KvCompactArgs a) {
     if (r >= used) return;
     const int64_t from = w.pages[r] * a.a.nb_page, to = r * a.b.nb_page;
     const int per = a.a.Hkv << (a.a.shift + a.cshift);               // pieces of a page in one pool
-    // every load before the first store, and none under a condition: one that might not happen is not asked for before its store
+    // every load before the first store, and none under a condition: one that might not happen is not asked for before its store (99 and 18 us)
     u32x4_t x[KV_SLICE / 256];
     char * dst[KV_SLICE / 256];
     #pragma unroll
