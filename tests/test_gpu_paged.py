@@ -249,6 +249,26 @@ def test_compact_moves_the_held_pages_and_renames_them(gpu, order, order2, dim, 
         q.check(full)
 
 
+@pytest.mark.parametrize("n_pages,page,heads,dim", [(4500, 1, 1, 64), (2048, 1, 2, 128), (2049, 2, 1, 64), (40, 64, 20, 128)])
+def test_compact_of_many_pages_or_large_ones(gpu, n_pages, page, heads, dim):
+    """on both sides of the sizes from which the ranks have a launch of their own"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=3, n_pages=n_pages, max_pages=n_pages // 2, page=page, heads=heads, dim=dim)
+    third = n_pages // 3 * page
+    assert p.append([(0, third), (1, third - 1), (2, third // 2)]) == 0
+    p.truncate([(0, third // 3), (1, 0)])
+    assert p.append([(1, third // 4)]) == 0
+    used = [x for x in range(n_pages) if p.count[x]]
+    name = {x: i for i, x in enumerate(used)}
+    for room in (len(used), len(used) + 300):
+        q = Pool(gpu, n_seq=3, n_pages=room, max_pages=n_pages // 2 + 1, page=page, heads=heads, dim=dim)
+        p.run(ctx.kv_compact_call(p.c, q.c))
+        q.rows, q.keys = [[name[x] for x in r] for r in p.rows], [list(x) for x in p.keys]
+        q.count = [p.count[x] for x in used] + [0] * (room - len(used))
+        q.content = {(i, j): None for i in range(len(used)) for j in range(page)}
+        q.check()
+
+
 # ---- attention ----------------------------------------------------------------------------------------------------------------
 
 

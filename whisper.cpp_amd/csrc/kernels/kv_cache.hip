@@ -397,7 +397,7 @@ extern "C" int mi355x_kv_fork(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n
 
 // ---------------------------------------------------------------------------------------------------------------
 // compact: the held pages' ranks (one workgroup, 5 us for 10000), then pages and table.  Bound by HBM: every held page is read and written once.  Half a
-// gigabyte in and out: 91 us = 5.0 TB/s; three megabytes 7 us.
+// gigabyte in and out: 91 us = 5.0 TB/s.
 // ---------------------------------------------------------------------------------------------------------------
 struct KvCompactArgs { kvc a, b; int cshift, slices, table_blocks; };
 __global__ void __launch_bounds__(KV_WG) k_kv_rank(const KvCompactArgs a) {
@@ -422,6 +422,24 @@ __global__ void __launch_bounds__(KV_WG) k_kv_rank(const KvCompactArgs a) {
     }
 }
 #define KV_SLICE 1024             // 16-byte pieces per workgroup
+// slice `slice` of page `p` to page r of the new pool
+__device__ __forceinline__ void kv_move(const KvCompactArgs & a, int p, int r, int slice) {
+    const int64_t from = p * a.a.nb_page, to = r * a.b.nb_page;
+    const int per = a.a.Hkv << (a.a.shift + a.cshift);               // pieces of a page in one pool
+    // every load before the first store, and none under a condition: one that might not happen is not asked for before its store (99 and 18 us)
+    u32x4_t x[KV_SLICE / 256];
+    char * dst[KV_SLICE / 256];
+    #pragma unroll
+    for (int e = 0; e < KV_SLICE / 256; e++) {
+        const int j0 = slice * KV_SLICE + e * 256 + threadIdx.x, j1 = min(j0, 2 * per - 1);
+        const bool isv = j1 >= per;
+        const int j = isv ? j1 - per : j1, ch = j & ((1 << a.cshift) - 1), row = j >> a.cshift, key = row & a.a.mask, head = row >> a.a.shift;
+        x[e] = *(const u32x4_t *) ((isv ? a.a.v : a.a.k) + from + head * a.a.nb_head + key * a.a.nb_key + ch * 16);
+        dst[e] = j0 < 2 * per ? (isv ? a.b.v : a.b.k) + to + head * a.b.nb_head + key * a.b.nb_key + ch * 16 : nullptr;
+    }
+    #pragma unroll
+    for (int e = 0; e < KV_SLICE / 256; e++) if (dst[e]) *(u32x4_t *) dst[e] = x[e];
+}
 __global__ void __launch_bounds__(256) k_kv_compact(const KvCompactArgs a) {
     const kv_work w = kv_work_of(a.a.work, a.a.n_seq, a.a.n_pages);
     const int used = w.flag[1];
@@ -440,21 +458,55 @@ __global__ void __launch_bounds__(256) k_kv_compact(const KvCompactArgs a) {
     const int64_t blk = blockIdx.x - a.table_blocks;
     const int r = (int) (blk / a.slices), slice = (int) (blk - (int64_t) r * a.slices);
     if (r >= used) return;
-    const int64_t from = w.pages[r] * a.a.nb_page, to = r * a.b.nb_page;
-    const int per = a.a.Hkv << (a.a.shift + a.cshift);               // pieces of a page in one pool
-    // every load before the first store, and none under a condition: one that might not happen is not asked for before its store (99 and 18 us)
-    u32x4_t x[KV_SLICE / 256];
-    char * dst[KV_SLICE / 256];
+    kv_move(a, w.pages[r], r, slice);
+}
+
+// few pages and few slices: every workgroup ranks the pages for itself, without the first launch (822 pages, 4 MB in and out: 4.1 us, two launches
+// 7.1); with more than 16 slices for each CU the ranks would be made again and again
+#define KV_SMALL_PAGES 2048
+#define KV_SMALL_SLICES 4096
+__global__ void __launch_bounds__(256) k_kv_compact_small(const KvCompactArgs a) {
+    constexpr int PER = KV_SMALL_PAGES / 256;
+    __shared__ int rank[KV_SMALL_PAGES], sum[4], mine;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, p0 = tid * PER;
+    int ref[PER], cnt = 0;
     #pragma unroll
-    for (int e = 0; e < KV_SLICE / 256; e++) {
-        const int j0 = slice * KV_SLICE + e * 256 + threadIdx.x, j1 = min(j0, 2 * per - 1);
-        const bool isv = j1 >= per;
-        const int j = isv ? j1 - per : j1, ch = j & ((1 << a.cshift) - 1), row = j >> a.cshift, key = row & a.a.mask, head = row >> a.a.shift;
-        x[e] = *(const u32x4_t *) ((isv ? a.a.v : a.a.k) + from + head * a.a.nb_head + key * a.a.nb_key + ch * 16);
-        dst[e] = j0 < 2 * per ? (isv ? a.b.v : a.b.k) + to + head * a.b.nb_head + key * a.b.nb_key + ch * 16 : nullptr;
+    for (int e = 0; e < PER; e++) ref[e] = a.a.ref[min(p0 + e, a.a.n_pages - 1)];
+    #pragma unroll
+    for (int e = 0; e < PER; e++) { if (p0 + e >= a.a.n_pages) ref[e] = 0; cnt += ref[e] > 0; }
+    int at = cnt;
+    #pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(at, o, 64); if (lane >= o) at += u; }
+    if (lane == 63) sum[wave] = at;
+    __syncthreads();
+    int used = 0;
+    at -= cnt;
+    #pragma unroll
+    for (int w = 0; w < 4; w++) { if (w < wave) at += sum[w]; used += sum[w]; }
+    if (used > a.b.n_pages) { if (blockIdx.x == 0 && tid == 0) atomicOr((unsigned *) a.b.status, MI355X_KV_OUT_OF_PAGES); return; }
+    const int blk = (int) blockIdx.x - a.table_blocks, r = blk / a.slices;
+    if (blk >= 0) {
+        if (r >= used) return;
+        #pragma unroll
+        for (int e = 0; e < PER; e++) if (ref[e] > 0 && at++ == r) mine = p0 + e;
+        __syncthreads();
+        kv_move(a, mine, r, blk - r * a.slices);
+        return;
     }
     #pragma unroll
-    for (int e = 0; e < KV_SLICE / 256; e++) if (dst[e]) *(u32x4_t *) dst[e] = x[e];
+    for (int e = 0; e < PER; e++) {
+        rank[p0 + e] = ref[e] > 0 ? at : -1;
+        if (ref[e] > 0) { if (blockIdx.x == 0) a.b.ref[at] = ref[e]; at++; }
+    }
+    __syncthreads();
+    const int64_t step = (int64_t) a.table_blocks * 256, i0 = (int64_t) blockIdx.x * 256 + tid, nt = (int64_t) a.b.n_seq * a.b.max_pages;
+    for (int64_t i = i0; i < nt; i += step) {
+        const int64_t s = i / a.b.max_pages, col = i - s * a.b.max_pages;
+        const int p = col < a.a.max_pages ? a.a.table[s * a.a.max_pages + col] : -1;
+        a.b.table[i] = p >= 0 && p < a.a.n_pages ? rank[p] : -1;
+    }
+    for (int64_t i = i0; i < a.b.n_seq; i += step) a.b.len[i] = a.a.len[i];
+    for (int64_t i = used + i0; i < a.b.n_pages; i += step) a.b.ref[i] = 0;
 }
 extern "C" int mi355x_kv_compact(mi355x_ctx * ctx, const mi355x_kv_cache * from, const mi355x_kv_cache * to) {
     KvCompactArgs a; int rc = kv_view(from, &a.a);
@@ -469,11 +521,16 @@ extern "C" int mi355x_kv_compact(mi355x_ctx * ctx, const mi355x_kv_cache * from,
     a.cshift = from->head_dim == 64 ? 3 : 4;
     const int64_t per = (int64_t) 2 * from->n_head_kv * from->page_size << a.cshift;
     a.slices = (int) ((per + KV_SLICE - 1) / KV_SLICE);
-    int64_t tb = ((int64_t) to->n_seq * to->max_pages + to->n_pages) / 2048 + 1;
+    const int64_t entries = (int64_t) to->n_seq * to->max_pages + to->n_pages;
+    int64_t tb = entries / 2048 + 1;
     a.table_blocks = (int) (tb > 1024 ? 1024 : tb);
     const int64_t pages = from->n_pages < to->n_pages ? from->n_pages : to->n_pages;     // at most so many are held and fit
     const int64_t blocks = a.table_blocks + pages * a.slices;
     if (per > INT32_MAX || blocks > INT32_MAX) return kv_refuse("kv_compact: pools too large for one launch");
+    if (from->n_pages <= KV_SMALL_PAGES && pages * a.slices <= KV_SMALL_SLICES) {
+        a.table_blocks = (int) (entries / 256 + 1 > 1024 ? 1024 : entries / 256 + 1);
+        return emit(ctx, "kv_compact", k_kv_compact_small, dim3((uint32_t) (a.table_blocks + pages * a.slices)), dim3(256), 0, a);
+    }
     rc = emit(ctx, "kv_rank", k_kv_rank, dim3(1), dim3(KV_WG), 0, a);
     return rc ? rc : emit(ctx, "kv_compact", k_kv_compact, dim3((uint32_t) blocks), dim3(256), 0, a);
 }
