@@ -37,6 +37,18 @@ __device__ __forceinline__ int last_at_most(const int * at, int n, int x) {
     return lo;
 }
 
+// the same by a whole wave, for an x that is one of the wave's: 64 entries at a look, one load's latency where a bisection has log2(n)
+__device__ __forceinline__ int last_at_most_wave(const int * at, int n, int x) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, step = 1;
+    while (step * 64 < n) step *= 64;
+    for (; step > 0; step /= 64) {
+        const int i = (int) min((int64_t) lo + (int64_t) lane * step, (int64_t) n - 1);
+        lo = min(lo + max(__popcll(__ballot(lo + (int64_t) lane * step < n && at[i] <= x)) - 1, 0) * step, n - 1);
+    }
+    return lo;
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // reset
 // ---------------------------------------------------------------------------------------------------------------
@@ -208,15 +220,29 @@ template <int NT, int U> struct kv_pieces {
     }
 };
 
-// byte offset of packed row r's place in the pools, -1 if the row belongs to no sequence
-__device__ __forceinline__ int64_t kv_place(const KvAppendArgs & a, const kv_work & w, int r) {
+// byte offset of packed row r's place in the pools (entry i's, if the row has one), -1 if it belongs to no sequence
+__device__ __forceinline__ int64_t kv_place(const KvAppendArgs & a, const kv_work & w, int r, int i) {
     if (r < a.cu[0] || r >= a.cu[a.n]) return -1;
-    const int i = last_at_most(a.cu, a.n, r), s = a.seq[i];
+    const int s = a.seq[i];
     if (s < 0) return -1;
     const int at = w.start[i] + r - a.cu[i];
     const int p = a.c.table[(int64_t) s * a.c.max_pages + (at >> a.c.shift)];
     if (p < 0 || p >= a.c.n_pages) return -1;                        // a table that the caller has overwritten
     return p * a.c.nb_page + (at & a.c.mask) * a.c.nb_key;
+}
+
+// the places of rows r0 .. r0 + nr - 1: each wave finds the entries of its rows (by turns), then a lane for each row follows it to its page
+template <int NT, int ROWS> __device__ __forceinline__ void kv_places(const KvAppendArgs & a, const kv_work & w, int r0, int nr, int64_t * place) {
+    constexpr int NW = NT / 64, PER = (ROWS + NW - 1) / NW;
+    static_assert(PER <= 64, "a lane for each of a wave's rows");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane * NW + wave;
+    int i = 0;
+    #pragma unroll
+    for (int q = 0; q < PER; q++) if (q * NW + wave < nr) {
+        const int found = last_at_most_wave(a.cu, a.n, r0 + q * NW + wave);
+        if (lane == q) i = found;
+    }
+    if (lane < PER && r < nr) place[r] = kv_place(a, w, r0 + r, i);
 }
 
 // the rows of entry i's last page that its sequence shared, into the page of its own
@@ -243,7 +269,7 @@ __global__ void __launch_bounds__(KV_WG) k_kv_reserve(const KvAppendArgs a) {
 // rows into their pages: rb rows per workgroup, whose places are looked up while the rows are on their way; behind them one workgroup per entry for shared
 // last pages.  Bound by HBM (rows in, rows out) once there are enough rows: with the two launches before it (9 us) 17321 rows of 8 heads of 128, 142 MB in
 // and out, 44 us, of which this is 28.7 (4.9 TB/s); four pieces of a thread at a time (eight: 46; places first, then the rows: 45, and 300 rows a sequence
-// 15.1 instead of 13.7).
+// 15.1 instead of 13.7; a bisection for each row: 32 rows 12.6, so 12.3).
 #define KV_U 4
 #define KV_RB 16
 __global__ void __launch_bounds__(256) k_kv_write(const KvAppendArgs a) {
@@ -254,7 +280,7 @@ __global__ void __launch_bounds__(256) k_kv_write(const KvAppendArgs a) {
     kv_pieces<256, KV_U> p;
     p.load(a, r0, count, threadIdx.x);
     if (w.flag[0] == 0) return;
-    if ((int) threadIdx.x < nr) at[threadIdx.x] = kv_place(a, w, r0 + threadIdx.x);
+    kv_places<256, KV_RB>(a, w, r0, nr, at);
     __syncthreads();
     p.store(a, at, count, threadIdx.x);
     for (int j0 = threadIdx.x + KV_U * 256; j0 < count; j0 += KV_U * 256) { p.load(a, r0, count, j0); p.store(a, at, count, j0); }
@@ -275,7 +301,7 @@ __global__ void __launch_bounds__(KV_WG) k_kv_append_small(const KvAppendArgs a)
     p.load(a, 0, count, threadIdx.x);
     if (!kv_reserve(a, w, seen, part, shared)) return;
     __syncthreads();                                                 // table and lists as they are now
-    if ((int) threadIdx.x < a.rows) at[threadIdx.x] = kv_place(a, w, threadIdx.x);
+    if ((int) threadIdx.x < a.rows) at[threadIdx.x] = kv_place(a, w, threadIdx.x, last_at_most(a.cu, a.n, threadIdx.x));
     if (shared[1]) for (int i = threadIdx.x >> 6; i < a.n; i += KV_WG / 64) kv_copy_shared<64>(a, w, i, threadIdx.x & 63);
     __syncthreads();
     p.store(a, at, count, threadIdx.x);
