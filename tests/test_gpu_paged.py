@@ -459,6 +459,14 @@ def test_attention_of_prompt_pieces_over_the_cache(gpu, kind, dim, kv_heads, hea
     packed_case(gpu, kind, kind, kind, dim, kv_heads, heads, [3, 1, 70, 9, 0, 40, 4], [200, 1, 70, 3, 33, 0, 131], page=page, order=order, causal=causal, window=window)
 
 
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("heads,dim,q_lens,k_lens", [(128, 64, [200, 3], [200, 3]), (65, 64, [130], [190]), (128, 128, [1, 0, 0, 0], [1500, 2, 0, 30]), (96, 128, [40, 30], [300, 290])])
+def test_more_heads_to_a_group_than_half_a_workgroup_has_rows(gpu, heads, dim, q_lens, k_lens, page):
+    """a row tile of 64 cannot hold one query of such a group, at lengths where smaller groups would get it"""
+    packed_case(gpu, "f16", "f16", "f16", dim, 1, heads, q_lens, k_lens, page=page)
+    packed_case(gpu, "bf16", "f32", "f32", dim, 1, heads, q_lens, k_lens, page=page, window=100)
+
+
 @pytest.mark.parametrize("max_q", [0, 1, 12, 64, 4000])
 @pytest.mark.parametrize("dim,heads", [(64, 1), (128, 4)])
 def test_what_the_caller_says_of_the_rows_never_changes_what_is_computed(gpu, dim, heads, max_q):

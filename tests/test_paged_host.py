@@ -133,3 +133,50 @@ def test_ctypes_mirrors_of_the_paged_structs(tmp_path):
         name, size, *offs = line.split()
         assert C.sizeof(probes[name]) == int(size)
         assert [getattr(probes[name], f[0]).offset for f in probes[name]._fields_] == [int(x) for x in offs]
+
+
+SWEEP = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import __graft_entry__ as graft
+graft.load_package()
+import ctypes as C
+from whisper_cpp_amd import kernels_api as ka
+blank = C.create_string_buffer(65536)
+mem = (C.c_char * 4096).from_buffer(bytearray(4096))
+at = (C.addressof(mem) + 63) // 64 * 64
+seen = set()
+for dim in (64, 128):
+    for kv_heads in (1, 2):
+        for group in range(1, 129):
+            for n, rows, keys, max_q in ((1, 200, 200, 0), (1, 1, 1000, 0), (4, 1, 8000, 0), (4, 1, 8000, 1), (1, 4000, 4000, 0), (1, 100, 300, 8), (16, 100000, 100000, 0), (9, 9, 90, 3)):
+                for cached in (False, True):
+                    H = kv_heads * group
+                    d = ka.AttnPackedDesc()
+                    d.q, d.dst = (ka.tensor(at, ka.F32, [dim, H, rows], [4, 4 * dim, 4 * dim * H]) for _ in range(2))
+                    d.k, d.v = (ka.tensor(at, ka.F16, [dim, kv_heads, keys], [2, 2 * dim, 2 * dim * kv_heads]) for _ in range(2))
+                    d.cu_q, d.n, d.scale, d.causal, d.max_q = at, n, 1.0, 1, max_q
+                    c = ka.KvCache()
+                    c.k, c.v, c.type, c.head_dim, c.n_head_kv, c.page_size, c.n_pages, c.n_seq, c.max_pages = at, at, ka.F16, dim, kv_heads, 16, 8, 16, -(-keys // 16)
+                    c.nb_key, c.nb_head, c.nb_page = 2 * dim, 32 * dim, 32 * dim * kv_heads
+                    c.table = c.len = c.ref = c.status = c.work = at
+                    if cached:
+                        d.cache = C.pointer(c)
+                    print(dim, H, kv_heads, n, rows, keys, max_q, cached, flush=True)
+                    seen.add(ka.lib().mi355x_attn_packed(C.cast(blank, C.c_void_p), C.byref(d)))
+print("answers:", *sorted(seen))
+"""
+
+
+def test_every_group_of_heads_finds_a_form_of_the_packed_attention():
+    """up to 128 query heads to a K/V head, in every branch of the choice: each call gets as far as its launch, which finds no device (a process of its own, which sees none)"""
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT
+    env = {**os.environ, "HIP_VISIBLE_DEVICES": "-1", "ROCR_VISIBLE_DEVICES": "-1"}
+    r = subprocess.run([sys.executable, "-c", SWEEP, str(ROOT)], env=env, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, timeout=300)
+    lines = r.stdout.strip().splitlines()
+    assert r.returncode == 0, (r.returncode, lines[-1:])
+    name, *answers = lines[-1].split()
+    assert name == "answers:" and answers and all(int(x) > 0 for x in answers), lines[-1]

@@ -350,6 +350,7 @@ template <typename O, int D, bool PAGED, int NW, int KG>
 static int launch_packed_as(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv) {
     static std::atomic<uint64_t> allowed{0};
     a.qt = 32 * NW / KG / a.G;
+    if (a.qt < 1) return kv_refuse("attn_packed: a group of more heads than a workgroup has rows");      // (launch_packed chooses a form that has them)
     const int64_t blocks = ((int64_t) a.rows_q / a.qt + a.n) * Hkv;
     if (blocks > INT32_MAX) return kv_refuse("attn_packed: too many rows for one launch");
     const uint32_t lds = (NW == 8 ? 3 * 3 * 64 : KG == 2 ? 3 * 64 : 3 * 32) * D * 2 + 16;
@@ -373,13 +374,14 @@ static int launch_packed(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv, int max_
     const int64_t few = (int64_t) a.n * Hkv * ((max_q * (int64_t) a.G + 15) / 16);   // workgroups of 16 rows
     if (max_q > 0 && (int64_t) max_q * a.G <= 256 && few <= ctx->n_cu && keys >= 256) return mi355x_attn_few_rows(ctx, a, __is_same(O, f16_ops) ? MI355X_TYPE_F16 : MI355X_TYPE_BF16, D, PAGED);
     const int64_t wide = rows * Hkv / 256;                           // workgroups of 256 rows, if all were full
+    const bool pairs = a.G <= 64;                                    // four waves, two on each tile's keys: 64 rows, which have to hold a group's heads
     if constexpr (D == 64) {
-        if (wide < 512 && keys >= 128) return launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv);
+        if (wide < 512 && keys >= 128 && pairs) return launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv);
         return launch_packed_as<O, D, PAGED, 4, 1>(ctx, a, Hkv);
     } else {
         const int64_t per = (rows + a.n - 1) / a.n;                  // of one sequence on the average
         const bool wedge = a.causal && a.window == 0 && keys <= 2 * (a.rows_q / a.n);
-        if (wide <= (wedge ? ctx->n_cu : ctx->n_cu / 2) && keys >= 256) return per <= 64 ? launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv) : launch_packed_as<O, D, PAGED, 8, 2>(ctx, a, Hkv);
+        if (wide <= (wedge ? ctx->n_cu : ctx->n_cu / 2) && keys >= 256) return per <= 64 && pairs ? launch_packed_as<O, D, PAGED, 4, 2>(ctx, a, Hkv) : launch_packed_as<O, D, PAGED, 8, 2>(ctx, a, Hkv);
         return keys <= 768 ? launch_packed_as<O, D, PAGED, 4, 1>(ctx, a, Hkv) : launch_packed_as<O, D, PAGED, 8, 1>(ctx, a, Hkv);
     }
 }
