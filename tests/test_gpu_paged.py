@@ -534,6 +534,62 @@ def test_the_largest_and_smallest_values_of_the_type(gpu):
         assert float(((out[0, 0].double() - want).abs() / want.abs().clamp_min(v.double().abs().mean(0) * 1e-2)).max()) < 100 * 40 * U["f32"]
 
 
+def equal_best_keys(torch, p, lens, kind, best, rng):
+    """Fills the keys of sequences 0 .. of `p` (already appended): `best` of them are the same key, the others zeros, so that scores are sums of one product and the best
+    ones are equal in any precision; returns (the queries' two values, the best keys' numbers, values [L, dim] of each sequence, all on the CPU)."""
+    a, b = (torch.tensor([x], dtype=torch.float64).to(dt(torch, kind)).item() for x in (rng.uniform(1, 2), rng.uniform(1, 2)))
+    at, values = [], []
+    for s, L in enumerate(lens):
+        keys = sorted(rng.sample(range(L), best))
+        for j in range(L):
+            x = p.rows[s][j // p.page], 0, j % p.page
+            p.k[x] = 0.0
+            if j in keys:
+                p.k[x[0], 0, x[2], 0] = a
+        at.append(keys)
+        values.append(torch.stack([x[1][0] for x in p.keys[s]]).double())
+    return a, b, at, values
+
+
+@pytest.mark.parametrize("kind,q_kind", [("f16", "f32"), ("f16", "f16"), ("bf16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("bits", range(18, 44, 2))
+def test_scores_up_to_the_ends_of_the_range(gpu, kind, q_kind, bits):
+    """Scores of about 2^bits in every way that the attentions run: a few equal best keys share the weight, whatever the products with the scale are rounded by.
+    The best weights are the same number w, so that the result is the mean of their values up to the sums' and the quotient's rounding: 8 * 2^-24 of the largest
+    value, with w rounded to the cache's type once (the same for all: 2 u(kind) of the largest value in the quotient), and the result's own rounding."""
+    ctx, ka, torch = gpu
+    rng = random.Random(bits)
+    lens, best = [70, 300, 33], 3
+    p = Pool(gpu, n_seq=3, n_pages=32, max_pages=20, page=16, heads=1, dim=64, kind=kind, seed=bits)
+    assert p.append(list(enumerate(lens)), kind) == 0
+    a, b, at, values = equal_best_keys(torch, p, lens, kind, best, rng)
+    scale, small = 2.0 ** bits * rng.uniform(1, 2) / (a * b), 2 * U[kind] + 8 * U["f32"]
+
+    def hold(out, s):
+        want = values[s][at[s]].mean(0)
+        tol = small * values[s][at[s]].abs().amax() + U["f32"] * want.abs()
+        assert float(((out.double().cpu() - want).abs() - tol).max()) <= 0, (s, out[:4], want[:4])
+
+    q = torch.zeros(3, 2, 64, device="cuda")
+    q[:, 0, 0], q[:, 1, 0] = b, b * 0.75                             # the second head's scores: other roundings of the same keys
+    q = q.to(dt(torch, q_kind))
+    out = torch.empty(3, 2, 64, device="cuda")
+    p.run(ctx.attn_paged_call(p.c, q, out, scale=scale))
+    for s in range(3):
+        hold(out[s, 0], s)
+        hold(out[s, 1], s)
+    for max_q, rows in ((8, 2), (0, 2), (0, 100)):                   # few rows, the packed kernel's small and its larger row tiles; not causal, so that all rows see all keys
+        for n in (1, 2, 3):
+            qr = torch.zeros(n * rows, 2, 64, device="cuda")
+            qr[:, 0, 0], qr[:, 1, 0] = b, b * 0.75
+            out = torch.empty(n * rows, 2, 64, device="cuda")
+            p.run(ctx.attn_packed_call(qr.to(dt(torch, q_kind)), out, p.ints([i * rows for i in range(n + 1)]), cache=p.c, scale=scale, causal=False, max_q=max_q))
+            for i in range(n):
+                for r in sorted({0, rows // 2, rows - 1}):
+                    hold(out[i * rows + r, 0], i)
+                    hold(out[i * rows + r, 1], i)
+
+
 def test_a_decode_loop_captured_into_a_graph_and_replayed(gpu):
     """append, attention, fork and truncate of a step captured once on the context's stream; every replay, with new lists and eager work of the program
     between the replays, equals the same step run eagerly on a second cache"""

@@ -247,7 +247,16 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
                 #pragma unroll
                 for (int e = 0; e < 16; e++) o[i][e] *= alpha;
         }
-        const float mc = (m == -INFINITY ? 0.0f : m * a.c2) - (__is_same(O, f16_ops) ? 7.0f : 0.0f);
+        // m * c2 is rounded before the scores' products meet it: no more than F32 scores are off by themselves, and within 2^+-0.07 up to 2^20, but beyond the
+        // range of the weights' type (F16 from 2^24 on, any type from 2^31 on) for larger ones.  Those take the difference first.
+        float mc = m == -INFINITY ? 0.0f : m * a.c2;
+        if (__any(fabsf(mc) > 0x1p20f)) {
+            const float m0 = m == -INFINITY ? 0.0f : m;
+            #pragma unroll
+            for (int e = 0; e < 16 * NB; e++) s[e >> 4][e & 15] -= m0;
+            mc = 0.0f;
+        }
+        mc -= __is_same(O, f16_ops) ? 7.0f : 0.0f;
         float sum = 0.0f;
         #pragma unroll
         for (int b = 0; b < NB; b++)

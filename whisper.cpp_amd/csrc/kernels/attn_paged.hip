@@ -277,10 +277,14 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
                     for (int r = 0; r < 4; r++) o[d][r] *= alpha;
             }
             // F16 weights are held times 2^15, so that small ones do not fall below its range; the factor cancels against the sum's
-            const float shift = sizeof(typename O::elem) == 2 && __is_same(O, f16_ops) ? m - 15.0f : m;
+            // (added to the difference, which is small where weights are not: m - 15 is another number than it says from 2^24 on)
             float p[8];
             #pragma unroll
-            for (int e = 0; e < 8; e++) { p[e] = __builtin_amdgcn_exp2f(x[e] - shift); l += p[e]; }
+            for (int e = 0; e < 8; e++) {
+                const float d = x[e] - m;
+                p[e] = __builtin_amdgcn_exp2f(__is_same(O, f16_ops) ? d + 15.0f : d);
+                l += p[e];
+            }
             vec8 pf[NT];
             split8<O, NT>(p, pf);
             // V^T as the first operand: this 16-lane group's keys 4 g4 + {0..3} and 16 + 4 g4 + {0..3}, dims 16 d + {0..15}
