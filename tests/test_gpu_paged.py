@@ -590,6 +590,25 @@ def test_scores_up_to_the_ends_of_the_range(gpu, kind, q_kind, bits):
                     hold(out[i * rows + r, 1], i)
 
 
+def test_scores_near_the_lowest_number_of_all(gpu):
+    """every score is -3.3e38: below any start that a running maximum could have but the lowest number itself"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=1, n_pages=4, max_pages=4, page=16, heads=1, dim=64, kind="bf16")
+    assert p.append([(0, 50)], "bf16") == 0
+    k, v = (x.reshape(-1, 64)[:50] for x in (p.k, p.v))
+    k.zero_()
+    k[:, 0] = 2.0 ** 120
+    q = torch.zeros(1, 1, 64, device="cuda")
+    q[..., 0] = -1.0
+    out, want = torch.empty(1, 1, 64, device="cuda"), v.double().mean(0)
+    tol = 50 * U["f32"] * v.double().abs().amax()                    # equal weights: powers of two, so the sums' and the quotient's rounding alone
+    for scale in (3.3e38 / 2.0 ** 120 / 1.4426950408889634, 3.39e38 / 2.0 ** 120 / 1.4426950408889634):
+        p.run(ctx.attn_paged_call(p.c, q, out, scale=scale))
+        assert float((out[0, 0].double() - want).abs().max()) <= tol
+        p.run(ctx.attn_packed_call(q, out, p.ints([0, 1]), cache=p.c, scale=scale))
+        assert float((out[0, 0].double() - want).abs().max()) <= tol
+
+
 def test_a_decode_loop_captured_into_a_graph_and_replayed(gpu):
     """append, attention, fork and truncate of a step captured once on the context's stream; every replay, with new lists and eager work of the program
     between the replays, equals the same step run eagerly on a second cache"""

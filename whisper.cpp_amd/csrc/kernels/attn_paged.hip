@@ -22,7 +22,7 @@
 #define TILE 32                        // keys of a tile: one 16x16x32 product over keys
 #define MIN_RUN 8                      // tiles of a run at least: two for each wave
 #define OVERHEAD 6                     // tiles: of a query in a run, see cost_of
-#define NEG_BIG (-3.0e38f)             // the running maximum's start: exp2(x - NEG_BIG) of a masked x = -inf is 0, not NaN
+#define NEG_BIG (-__FLT_MAX__)         // the running maximum's start, no more than any score: exp2(x - NEG_BIG) of a masked x = -inf is 0, not NaN
 
 struct PagedArgs {
     kvc c;
