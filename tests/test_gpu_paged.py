@@ -506,6 +506,34 @@ def test_infinities_in_the_first_and_last_key_of_one_token_stay_what_they_are(gp
     assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("kind,dim,page", [("f16", 64, 4), ("bf16", 128, 16), ("f16", 128, 32)])
+@pytest.mark.parametrize("max_q,rows", [(0, 70), (0, 1), (8, 3)])
+def test_pages_before_the_window_may_be_gone(gpu, kind, dim, page, max_q, rows):
+    """columns of the table that lie wholly before the window hold no page: not an error, in either attention; one that a row sees is"""
+    ctx, ka, torch = gpu
+    keys, window = 401, 90
+    p = Pool(gpu, n_seq=1, n_pages=-(-keys // page), max_pages=-(-keys // page), page=page, heads=2, dim=dim, kind=kind)
+    assert p.append([(0, keys)], kind) == 0
+    q = torch.randn(rows, 4, dim, generator=p.gen, device="cuda").to(dt(torch, kind))
+    whole, out = torch.empty(rows, 4, dim, device="cuda"), torch.empty(rows, 4, dim, device="cuda")
+    packed = lambda to: ctx.attn_packed_call(q, to, p.ints([0, rows]), cache=p.c, scale=0.1, window=window, max_q=max_q)  # noqa: E731
+    paged = lambda to: ctx.attn_paged_call(p.c, q[:1], to[:1], scale=0.1, window=window)  # noqa: E731
+    first = keys - rows - window + 1                                 # of the keys that the first row of the packed call sees
+    for call, seen in ((packed, first), (paged, keys - window)):
+        p.run(call(whole))
+        gone = seen // page
+        assert gone > 0
+        p.table[0, :gone] = -1
+        p.run(call(out))
+        assert int(p.status) == 0
+        assert torch.equal(out[:1] if call is paged else out, whole[:1] if call is paged else whole)
+        p.table[0, gone] = -1
+        p.run(call(out))
+        assert int(p.status) == ka.KV_BAD_ARG
+        p.status.zero_()
+        p.table[0] = p.ints(p.rows[0])
+
+
 @pytest.mark.parametrize("page,max_q,ks", [(0, 0, [3, 40]), (16, 0, [3, 40]), (0, 8, [3, 600]), (16, 8, [3, 600])])
 @pytest.mark.parametrize("causal", [True, False])
 def test_a_window_beyond_every_length_is_none(gpu, page, max_q, ks, causal):

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
         for (int e = 0; e < NL; e++) {
             const int key = (T0 + t) * KT + skey + e * RPL;
             if (PAGED) {
-                bad |= (unsigned) pg[e] >= (unsigned) a.c.n_pages && key <= b_last;
+                bad |= (unsigned) pg[e] >= (unsigned) a.c.n_pages && key >= b_first && key <= b_last;     // (a page that no row sees may be gone)
                 at_k[e] = (int64_t) ((uint64_t) (uint32_t) min(max(pg[e], 0), a.c.n_pages - 1) * nb_page + (uint64_t) (uint32_t) (key & a.c.mask) * nb_key);
             } else at_k[e] = (int64_t) ((uint64_t) (uint32_t) min(key, L - 1) * nb_key);
         }
