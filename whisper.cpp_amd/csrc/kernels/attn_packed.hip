@@ -84,7 +84,9 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
     for (int i = 0; i < NI; i++)
         #pragma unroll
         for (int e = 0; e < 16; e++) o[i][e] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
+    constexpr float lift = __is_same(O, f16_ops) ? 7.0f : 0.0f;
+    float m = -INFINITY, l = 0.0f, mc = -lift;
+    bool big = false;                                                 // some row's maximum is so large that the scores meet it before their products with c2 are made
 
     // staging: thread -> key tid / PCS (+ RPL), piece tid % PCS.  A tile's keys behind the last are other rows of the pool or the last row again: no
     // row sees them, and what of their values is not finite is taken out below.  A tile's places are made once, for its keys, and kept for its values.
@@ -246,17 +248,17 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
             for (int i = 0; i < NI; i++)
                 #pragma unroll
                 for (int e = 0; e < 16; e++) o[i][e] *= alpha;
+            // m * c2 is rounded before the scores' products meet it: no more than F32 scores are off by themselves, and within 2^+-0.07 up to 2^20, but beyond
+            // the range of the weights' type (F16 from 2^24 on, any type from 2^31 on) for larger ones.  Those take the difference first.
+            mc = m == -INFINITY ? 0.0f : m * a.c2;
+            big = __any(fabsf(mc) > 0x1p20f);
+            mc = (big ? 0.0f : mc) - lift;
         }
-        // m * c2 is rounded before the scores' products meet it: no more than F32 scores are off by themselves, and within 2^+-0.07 up to 2^20, but beyond the
-        // range of the weights' type (F16 from 2^24 on, any type from 2^31 on) for larger ones.  Those take the difference first.
-        float mc = m == -INFINITY ? 0.0f : m * a.c2;
-        if (__any(fabsf(mc) > 0x1p20f)) {
+        if (__builtin_expect(big, 0)) {
             const float m0 = m == -INFINITY ? 0.0f : m;
             #pragma unroll
             for (int e = 0; e < 16 * NB; e++) s[e >> 4][e & 15] -= m0;
-            mc = 0.0f;
         }
-        mc -= __is_same(O, f16_ops) ? 7.0f : 0.0f;
         float sum = 0.0f;
         #pragma unroll
         for (int b = 0; b < NB; b++)
