@@ -377,7 +377,7 @@ MI355X_API int mi355x_kv_compact(mi355x_ctx * ctx, const mi355x_kv_cache * from,
  *   dst[:, h, i] = softmax_j(scale * q[:, h, i] . k_j) v_j     head h reads K/V head h / (n_head / n_head_kv)
  * An empty sequence and an entry of -1 give zeros.  q, dst: [head_dim, n_head, n], F32 / F16 / BF16, nb[0] = element, 16-byte aligned.  F32 queries
  * count as such (split into 2 or 3 terms of the cache's type, |q| <= 65504 with F16 caches), sums and softmax are F32.  Rows past a sequence's end
- * and before its window are never read.  max_len: what the caller knows of the lengths (0: nothing; the table's width); it decides how far the work
+ * and before its window are never read.  An infinity among the values that a query sees is the result's, however small its weight.  max_len: what the caller knows of the lengths (0: nothing; the table's width); it decides how far the work
  * is split over the keys, longer sequences are still complete.  work: mi355x_attn_paged_work_bytes(...) bytes of device memory (NULL if that is
  * 0); calls that may run at the same time need their own.  A page number outside the pool is reported in *status (that row's result means nothing). */
 typedef struct mi355x_attn_paged_desc {
@@ -398,7 +398,8 @@ MI355X_API int    mi355x_attn_paged(mi355x_ctx * ctx, const mi355x_kv_cache * c,
  * keys, row r sees the keys j <= L - Q + r (causal; all otherwise), and of them those with j > L - Q + r - window if window > 0.  A row
  * that sees nothing is zero; rows behind cu_q[n] are left as they are.  q, dst: [head_dim, n_head, rows]; k, v: [head_dim, n_head_kv, rows], F16 or
  * BF16 (64 or 128 dims), strides multiples of 16 bytes.  q F32 / F16 / BF16 is rounded to k's type as in mi355x_flash_attn_ext, weights too; sums and
- * softmax are F32; dst F32 / F16 / BF16.  Keys that a row does not see never reach it, whatever they hold.  max_q: an upper bound of the rows of
+ * softmax are F32; dst F32 / F16 / BF16.  Keys that a row does not see never reach it, whatever they hold; an infinity
+ * among the values that it does see is the result's, however small its weight.  max_q: an upper bound of the rows of
  * one sequence as far as the caller knows it (0: unknown); it decides how the rows are cut, longer sequences are still complete. */
 typedef struct mi355x_attn_packed_desc {
     mi355x_tensor   q, k, v, dst;  /* k, v: unused with a cache */

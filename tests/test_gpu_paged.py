@@ -506,6 +506,69 @@ def test_infinities_in_the_first_and_last_key_of_one_token_stay_what_they_are(gp
     assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("kind,io", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("dim,heads,rows,keys,max_q", [(64, 2, 1, 200, 1), (64, 2, 1, 1501, 1), (128, 2, 1, 3001, 1),              # one token: whole, split
+                                                       (64, 2, 8, 1201, 8), (128, 2, 8, 1201, 8),                                 # packed: few rows
+                                                       (64, 2, 8, 120, 0), (128, 2, 8, 200, 0), (64, 2, 40, 300, 0), (128, 2, 40, 300, 0), (128, 2, 100, 400, 0), (128, 16, 2200, 2300, 0)])
+def test_an_infinity_stays_one_however_small_its_weight(gpu, kind, io, dim, heads, rows, keys, max_q):
+    """infinities in tiles that every row sees whole, in keys whose weights are far below the smallest number of the cache's type, or of any: the exact weight is none
+    of 0, so the value's infinity is the result's; a NaN and two opposite ones make a NaN; all other dims have their values"""
+    ctx, ka, torch = gpu
+    page = 16
+    p = Pool(gpu, n_seq=1, n_pages=-(-keys // page), max_pages=-(-keys // page), page=page, heads=heads, dim=dim, kind=kind)
+    assert p.append([(0, keys)], kind) == 0
+    q = torch.full((rows, heads, dim), dim ** -0.5, device="cuda").to(dt(torch, io))
+    scale, inf = dim ** -0.5, float("inf")
+    at = lambda key: (p.rows[0][key // page], slice(None), key % page)  # noqa: E731
+    p.k.mul_(0.5)
+    low = [40, 41, 42, 64, 71]                                       # 60 and 400 below the others' scores (they are of about 0.5)
+    for key, depth in zip(low, (60.0, 400.0, 60.0, 60.0, 400.0)):
+        p.k[at(key)] = -depth / dim ** 0.5 / scale / dim ** 0.5
+    top = keys - rows - 5
+    p.k[at(top)] = 250.0 / dim ** 0.5 / scale / dim ** 0.5 if keys > 1000 else 0.5      # a maximum that comes late and leaves nothing of the others
+
+    def run():
+        out = torch.empty(rows, heads, dim, device="cuda")
+        if max_q == 1:
+            work = torch.empty(max(16, ka.attn_paged_work_bytes(p.c, 1, heads, 0)), dtype=torch.uint8, device="cuda")
+            p.run(ctx.attn_paged_call(p.c, q, out, scale=scale, work=work))
+            return [out]
+        p.run(ctx.attn_packed_call(q, out, p.ints([0, rows]), cache=p.c, scale=scale, max_q=max_q))
+        flat = [x.transpose(1, 2).reshape(-1, heads, dim)[:keys].contiguous() if p.rows[0] == list(range(len(p.rows[0]))) else None for x in (p.k, p.v)]
+        out2 = torch.empty_like(out)
+        p.run(ctx.attn_packed_call(q, out2, p.ints([0, rows]), k=flat[0], v=flat[1], cu_k=p.ints([0, keys]), scale=scale, max_q=max_q))
+        return [out, out2]
+
+    clean = run()
+    size = float(p.v[: -(-keys // page)].float().nan_to_num(0.0).abs().max())
+    for d, (a, x) in enumerate(((0, inf), (1, -inf), (1, inf), (3, -inf), (4, inf), (2, float("nan")), (0, inf), (3, inf))):
+        p.v[at(low[a])][..., d] = x
+    p.v[at(low[4])][..., 6] = -inf                                   # with +inf in key 40: NaN
+    for out, was in zip(run(), clean):
+        assert out[..., [0, 2, 4, 7]].isposinf().all() and out[..., [1, 3]].isneginf().all() and out[..., [5, 6]].isnan().all()
+        assert float((out[..., 8:] - was[..., 8:]).abs().max()) <= (keys + 32) * U["f32"] * size
+
+
+@pytest.mark.parametrize("kind,io", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("bf16", "f16")])
+@pytest.mark.parametrize("dim,keys,page", [(64, 200, 16), (128, 300, 64), (64, 2501, 16), (128, 3001, 64)])
+def test_infinities_of_values_under_one_token(gpu, kind, io, dim, keys, page):
+    """of ordinary weights, however many terms these are split into"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=1, n_pages=-(-keys // page), max_pages=-(-keys // page), page=page, heads=2, dim=dim, kind=kind)
+    assert p.append([(0, keys)], kind) == 0
+    q = torch.randn(1, 4, dim, generator=p.gen, device="cuda").to(dt(torch, io))
+    work = torch.empty(max(16, ka.attn_paged_work_bytes(p.c, 1, 4, 0)), dtype=torch.uint8, device="cuda")
+    clean, out = torch.empty(1, 4, dim, device="cuda"), torch.empty(1, 4, dim, device="cuda")
+    p.run(ctx.attn_paged_call(p.c, q, clean, scale=1 / dim, work=work))
+    inf = float("inf")
+    for key, d, x in ((33, 3, inf), (50, 4, -inf), (70, 7, float("nan")), (90, 3, inf), (90, 9, -inf), (150, 9, inf)):
+        p.v[p.rows[0][key // page], :, key % page, d] = x
+    p.run(ctx.attn_paged_call(p.c, q, out, scale=1 / dim, work=work))
+    assert out[..., 3].isposinf().all() and out[..., 4].isneginf().all() and out[..., [7, 9]].isnan().all()
+    rest = [d for d in range(dim) if d not in (3, 4, 7, 9)]
+    assert torch.equal(out[..., rest], clean[..., rest])
+
+
 @pytest.mark.parametrize("kind,dim,page", [("f16", 64, 4), ("bf16", 128, 16), ("f16", 128, 32)])
 @pytest.mark.parametrize("max_q,rows", [(0, 70), (0, 1), (8, 3)])
 def test_pages_before_the_window_may_be_gone(gpu, kind, dim, page, max_q, rows):

@@ -348,12 +348,31 @@ __global__ void __launch_bounds__(64 * NW, 2) k_attn_packed(const PackedArgs a) 
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (r < nrow) {
+        const int os = a.o_type == MI355X_TYPE_F32 ? 4 : 2;
         char * op = a.o + (int64_t) (job.r0 + qi) * a.o_nb2 + (int64_t) (hk * a.G + g) * a.o_nb1;
+        float all = 0.0f;
         #pragma unroll
         for (int i = 0; i < NI; i++)
             #pragma unroll
-            for (int e = 0; e < 4; e++)
-                store4(op + (32 * i + 8 * e + 4 * hf) * (a.o_type == MI355X_TYPE_F32 ? 4 : 2), a.o_type, o[i][4*e] * inv, o[i][4*e+1] * inv, o[i][4*e+2] * inv, o[i][4*e+3] * inv);
+            for (int e = 0; e < 4; e++) {
+                const float y0 = o[i][4*e] * inv, y1 = o[i][4*e+1] * inv, y2 = o[i][4*e+2] * inv, y3 = o[i][4*e+3] * inv;
+                all += y0 + y1 + y2 + y3;
+                store4(op + (32 * i + 8 * e + 4 * hf) * os, a.o_type, y0, y1, y2, y3);
+            }
+        if (__builtin_expect(all != all && l == l, 0)) {              // some may be NaN that are not: the values decide (kinds_of)
+            #pragma unroll 1
+            for (int d = 4 * hf; d < D; d += 8) {
+                const char * at = a.c.v + hk * a.c.nb_head + d * 2;
+                uint32_t kinds[4] = { 0, 0, 0, 0 };
+                #pragma unroll 1
+                for (int key = first; key <= last; key++) {
+                    if (PAGED) kinds_of<O>(at + min(max(row[key >> a.c.shift], 0), a.c.n_pages - 1) * a.c.nb_page + (key & a.c.mask) * a.c.nb_key, kinds);
+                    else kinds_of<O>(at + (int64_t) (k0 + key) * a.c.nb_key, kinds);
+                }
+                #pragma unroll
+                for (int n = 0; n < 4; n++) if (kinds[n]) store1(op + (d + n) * os, a.o_type, kinds_value(kinds[n]));
+            }
+        }
     }
 }
 

@@ -72,8 +72,9 @@ template <int D> __device__ __forceinline__ int v_swap(int key) { return D == 12
 
 enum { SMALL_PAGES, BIG_PAGES, ROWS };                   // where K and V lie: pages of fewer than 32 keys; 32 and more (a tile lies in one); packed rows
 
+// (registers: 64 dims and 16-bit queries fit four waves to a SIMD, if only just)
 template <typename O, int D, int NT, int SRC, bool PACKED>
-__global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
+__global__ void __launch_bounds__(512, D == 64 && NT == 1 && !PACKED ? 4 : 2) k_attn_paged(const PagedArgs a) {
     typedef typename O::vec8 vec8;
     constexpr int KK = D / 32;                           // 32-dim pieces of a key
     constexpr int NV = D / 16;                           // V loads of a tile; 16-dim blocks of the result
@@ -332,6 +333,18 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     l += lane_xor16(l);
     l += lane_xor32(l);
 
+    // a NaN among row h's sums of dims d .., where the row's weights are numbers: the values decide (kinds_of)
+    auto settle = [&](int h, int d, floatx4 & r) {
+        const int own_h = own + q_of(h), k_last = PACKED && a.causal ? min(own_h, sp.hi - 1) : sp.hi - 1, k_first = PACKED && a.window > 0 ? max(own_h - a.window + 1, 0) : sp.lo;
+        uint32_t kinds[4] = { 0, 0, 0, 0 };
+        #pragma unroll 1
+        for (int key = max(k_first, t0 * TILE); key <= min(k_last, t1 * TILE - 1); key++) {
+            if (SRC == ROWS) kinds_of<O>(a.c.v + hk * a.c.nb_head + (int64_t) (k0 + key) * a.c.nb_key + d * 2, kinds);
+            else kinds_of<O>(a.c.v + hk * a.c.nb_head + min(max(row[key >> a.c.shift], 0), a.c.n_pages - 1) * a.c.nb_page + (key & a.c.mask) * a.c.nb_key + d * 2, kinds);
+        }
+        #pragma unroll
+        for (int n = 0; n < 4; n++) if (kinds[n]) r[n] = kinds_value(kinds[n]);
+    };
     // join the waves: their (m, l) and O^T over the dead V areas, dim-major for the writer's runs
     __syncthreads();
     float * ml = (float *) lds, * ol = ml + waves * 32;
@@ -352,6 +365,8 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
             #pragma unroll
             for (int e = 0; e < 4; e++) r[e] += f * x[e];
         }
+        const float all = r[0] + r[1] + r[2] + r[3];
+        if (__builtin_expect(all != all && L == L, 0)) settle(h, d, r);
         if (whole) {
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             store4(a.o + (int64_t) (i + q_of(h)) * a.o_nb2 + (int64_t) (h0 + h_of(h)) * a.o_nb1 + d * (a.o_type == MI355X_TYPE_F32 ? 4 : 2), a.o_type, r[0] * inv, r[1] * inv, r[2] * inv, r[3] * inv);
@@ -369,6 +384,9 @@ __global__ void __launch_bounds__(512, 2) k_attn_paged(const PagedArgs a) {
     }
     if (SRC != ROWS && __any(bad) && lane == 0) atomicOr((unsigned *) a.c.status, MI355X_KV_BAD_ARG);
 }
+
+// the factor of a part whose maximum is so far below the whole's: never zero, which would make a NaN of an infinity in the part
+__device__ __forceinline__ float part_weight(float below) { return fmaxf(__builtin_amdgcn_exp2f(below), 0x1p-126f); }
 
 // Joins the parts of one query and head, where it has several; zeros where it has none.  D/4 threads take a part's sums, 1024/D parts at a time.
 template <int D, int NT>
@@ -393,7 +411,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const PagedArgs a) {
         #pragma unroll
         for (int u = 0; u < 4; u++) {
             if (s0 + u * NG >= n) break;
-            const float mn = fmaxf(M, m[u]), f0 = __builtin_amdgcn_exp2f(M - mn), f1 = __builtin_amdgcn_exp2f(m[u] - mn);
+            const float mn = fmaxf(M, m[u]), f0 = part_weight(M - mn), f1 = part_weight(m[u] - mn);
             M = mn; L = L * f0 + l[u] * f1;
             #pragma unroll
             for (int e = 0; e < 4; e++) r[e] = r[e] * f0 + x[u][e] * f1;
@@ -411,7 +429,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const PagedArgs a) {
     for (int e = 0; e < 4; e++) r[e] = 0.0f;
     #pragma unroll
     for (int w = 0; w < NG; w++) {
-        const float f = __builtin_amdgcn_exp2f(top[w] - T);
+        const float f = part_weight(top[w] - T);
         const floatx4 x = *(const floatx4 *) &red[w][d];
         L += f * lsum[w];
         #pragma unroll

@@ -109,6 +109,12 @@ __device__ __forceinline__ void store4(char * p, int type, float a, float b, flo
     else { typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4))); bf16x4_t h; h[0] = (__bf16) a; h[1] = (__bf16) b; h[2] = (__bf16) c; h[3] = (__bf16) d; *(bf16x4_t *) p = h; }
 }
 
+__device__ __forceinline__ void store1(char * p, int type, float a) {
+    if (type == MI355X_TYPE_F32) *(float *) p = a;
+    else if (type == MI355X_TYPE_F16) *(half_t *) p = (half_t) a;
+    else *(__bf16 *) p = (__bf16) a;
+}
+
 // ---- packed rows (attn_packed.hip, and attn_paged.hip's kernel for few rows) ----
 struct PackedArgs {
     kvc c;                             // PAGED: the cache.  Otherwise k, v and their strides in nb_key (rows) and nb_head
@@ -167,5 +173,20 @@ __device__ __forceinline__ float put_back(float count) {
     const int n = (int) count;
     return ((n & 127) ? INFINITY : 0.0f) + ((n & 0x3F80) ? -INFINITY : 0.0f) + (n >= 16384 ? NAN : 0.0f);
 }
+
+// ---- infinities among the values that a row sees ----
+// In the products, weights have 16 bits (or are sums of such terms): a weight below their range times an infinity is a NaN where it should be an infinity, and so are
+// two terms of one weight that have other signs.  The kernels leave it at that, and the writer of a result that came out a NaN, though the row's weights are numbers,
+// looks at the values itself: a bit for an infinity, a negative one, a NaN among four values (`at`: 8 bytes)
+template <typename O> __device__ __forceinline__ void kinds_of(const char * at, uint32_t * kinds) {
+    const uint32_t top = __is_same(O, f16_ops) ? 0x7C00 : 0x7F80;
+    const uint2 w = *(const uint2 *) at;
+    #pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t x = (e < 2 ? w.x : w.y) >> 16 * (e & 1) & 0xFFFF;
+        if ((x & top) == top) kinds[e] |= (x & 0x7FFF) != top ? 4u : x & 0x8000 ? 2u : 1u;
+    }
+}
+__device__ __forceinline__ float kinds_value(uint32_t kinds) { return kinds == 1 ? INFINITY : kinds == 2 ? -INFINITY : NAN; }
 
 #endif
