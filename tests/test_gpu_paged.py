@@ -569,6 +569,34 @@ def test_infinities_of_values_under_one_token(gpu, kind, io, dim, keys, page):
     assert torch.equal(out[..., rest], clean[..., rest])
 
 
+@pytest.mark.parametrize("kind,io", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("bf16", "f16")])
+@pytest.mark.parametrize("dim,keys,page", [(64, 200, 16), (128, 300, 64), (64, 2501, 16), (128, 3001, 64)])
+def test_infinities_of_keys_under_one_token(gpu, kind, io, dim, keys, page):
+    """a key whose score is -inf weighs nothing, one of +inf or NaN makes the row a NaN, however many terms the query is split into"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=1, n_pages=-(-keys // page), max_pages=-(-keys // page), page=page, heads=2, dim=dim, kind=kind)
+    assert p.append([(0, keys)], kind) == 0
+    q = torch.randn(1, 4, dim, generator=p.gen, device="cuda").abs_().add_(0.01).to(dt(torch, io))
+    at = lambda key: (p.rows[0][key // page], slice(None), key % page)  # noqa: E731
+    work = torch.empty(max(16, ka.attn_paged_work_bytes(p.c, 1, 4, 0)), dtype=torch.uint8, device="cuda")
+
+    def run():
+        out = torch.empty(1, 4, dim, device="cuda")
+        p.run(ctx.attn_paged_call(p.c, q, out, scale=1 / dim, work=work))
+        return out
+
+    for key in (0, 45, 100, keys - 1):
+        p.k[at(key)][..., 5] = float("-inf")
+        p.v[at(key)] = 1e4                                           # weighs nothing
+    flat = [x[: -(-keys // page)].transpose(1, 2).reshape(-1, 2, dim)[:keys].cpu() for x in (p.k, p.v)]
+    see = torch.tensor([j not in (0, 45, 100, keys - 1) for j in range(keys)])
+    o, tol = expect(torch, q[0].cpu(), *flat, see, 1 / dim, kind, io, "f32", False, io == kind)
+    same(torch, run()[0], o, tol)
+    for x in (float("inf"), float("nan")):
+        p.k[at(60)][..., 8] = x
+        assert run().isnan().all()
+
+
 @pytest.mark.parametrize("kind,dim,page", [("f16", 64, 4), ("bf16", 128, 16), ("f16", 128, 32)])
 @pytest.mark.parametrize("max_q,rows", [(0, 70), (0, 1), (8, 3)])
 def test_pages_before_the_window_may_be_gone(gpu, kind, dim, page, max_q, rows):

@@ -218,14 +218,16 @@ __global__ void __launch_bounds__(512, D == 64 && NT == 1 && !PACKED ? 4 : 2) k_
             const bool more = t + waves < t1;
             uint32_t put = v_put, get = v_get;
             asm volatile("" : "+v"(put), "+v"(get));                 // the places are made again in each step: kept for all steps they would cost a wave per SIMD in registers
-            floatx4 s[2];
+            floatx4 s[2], rest[2];                                   // the first terms' products, and the others'
             #pragma unroll
             for (int b = 0; b < 2; b++) {
-                s[b] = floatx4{ 0, 0, 0, 0 };
+                s[b] = rest[b] = floatx4{ 0, 0, 0, 0 };
                 #pragma unroll
-                for (int n = NT - 1; n >= 0; n--)
+                for (int n = NT - 1; n > 0; n--)
                     #pragma unroll
-                    for (int kk = 0; kk < KK; kk++) s[b] = O::mfma16(kr[b][kk], qf[n][kk], s[b]);
+                    for (int kk = 0; kk < KK; kk++) rest[b] = O::mfma16(kr[b][kk], qf[n][kk], rest[b]);
+                #pragma unroll
+                for (int kk = 0; kk < KK; kk++) s[b] = O::mfma16(kr[b][kk], qf[0][kk], s[b]);
             }
             if (more) { pg = checked(t + waves, pg); fetch_k(t + waves, pg); }
             // V into this wave's area.  Zero times an infinity or a NaN is none: where some row does not see all of the tile, they are taken out here,
@@ -264,6 +266,8 @@ __global__ void __launch_bounds__(512, D == 64 && NT == 1 && !PACKED ? 4 : 2) k_
             #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int key = t * TILE + 16 * (e >> 2) + 4 * g4 + (e & 3);
+                // (an infinite key: the first term's sign is the query's, the others' need not be)
+                if (NT > 1) s[e >> 2][e & 3] += __builtin_amdgcn_fmed3f(rest[e >> 2][e & 3], -0x1p126f, 0x1p126f);
                 x[e] = key >= first && key <= last ? s[e >> 2][e & 3] * a.c2 : -INFINITY;
                 top = fmaxf(top, x[e]);
             }
