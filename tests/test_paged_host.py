@@ -119,6 +119,55 @@ def test_python_descriptions_refuse_arrays_that_do_not_fit():
             ka.kv_cache(**{**ok, **change})
 
 
+def test_calls_refuse_arrays_that_are_not_on_the_contexts_device():
+    """host memory, or another device's, is no memory for a kernel: refused where the call is made up, before there is anything to launch"""
+    import torch
+    ctx = object.__new__(ka.Ctx)
+    ctx.h, ctx.device = CTX, 0
+
+    class On:
+        """a host array that says it lies on a device"""
+        def __init__(self, t, device):
+            self.t, self.device = t, torch.device(device)
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    def arrays(device):
+        on = lambda t: On(t, device)  # noqa: E731
+        i = lambda *n: on(torch.zeros(*n, dtype=torch.int32))  # noqa: E731
+        k = torch.zeros(8, 2, 16, 64, dtype=torch.float16)
+        a = dict(cache=ka.kv_cache(on(k), on(k.clone()), i(4, 4), i(4), i(8), i(1), on(torch.zeros(ka.kv_work_bytes(4, 8), dtype=torch.uint8))))
+        a.update(seq=i(3), cu=i(4), rows=on(torch.zeros(3, 2, 64)), kv=on(torch.zeros(3, 2, 64, dtype=torch.float16)), work=on(torch.zeros(64, dtype=torch.uint8)))
+        return a
+
+    calls = {                                                        # of each call, the names of its arrays
+        "reset": (lambda a: ctx.kv_reset_call(a["cache"]), "cache"),
+        "append": (lambda a: ctx.kv_append_call(a["cache"], a["seq"], a["cu"], a["k"], a["v"]), "cache seq cu k v"),
+        "truncate": (lambda a: ctx.kv_truncate_call(a["cache"], a["seq"], a["keep"]), "cache seq keep"),
+        "fork": (lambda a: ctx.kv_fork_call(a["cache"], a["src"], a["dst"]), "cache src dst"),
+        "compact": (lambda a: ctx.kv_compact_call(a["cache"], a["to"]), "cache to"),
+        "paged": (lambda a: ctx.attn_paged_call(a["cache"], a["q"], a["out"], seq=a["seq"], work=a["work"]), "cache q out seq work"),
+        "packed": (lambda a: ctx.attn_packed_call(a["q"], a["out"], a["cu"], k=a["kv"], v=a["v16"], cu_k=a["cu_k"]), "q out cu kv v16 cu_k"),
+        "packed over a cache": (lambda a: ctx.attn_packed_call(a["q"], a["out"], a["cu"], cache=a["cache"], seq=a["seq"]), "q out cu cache seq"),
+    }
+    same = dict(k="rows", v="rows", q="rows", out="rows", keep="seq", src="seq", dst="seq", to="cache", v16="kv", cu_k="cu")
+    of = lambda a, name: a[same.get(name, name)]  # noqa: E731
+    good = arrays("cuda:0")
+    for what, (make, names) in calls.items():
+        mine = {name: of(good, name) for name in names.split()}
+        make(mine)                                                   # (made up, not called)
+        for other in ("cpu", "cuda:1"):
+            bad = arrays(other)
+            for name in names.split():
+                with pytest.raises(ValueError, match="context's device"):
+                    make({**mine, name: of(bad, name)})
+    k = torch.zeros(8, 2, 16, 64, dtype=torch.float16)
+    i = lambda *n: torch.zeros(*n, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError, match="one device"):
+        ka.kv_cache(k, k.clone(), On(i(4, 4), "cuda:0"), i(4), i(8), i(1), torch.zeros(ka.kv_work_bytes(4, 8), dtype=torch.uint8))
+
+
 def test_ctypes_mirrors_of_the_paged_structs(tmp_path):
     import subprocess
     from conftest import ROOT

@@ -259,6 +259,12 @@ def _ints(t, n: int, what: str):
     return t.data_ptr()
 
 
+def _device(t):
+    """of an array, as (type, number); None where it does not say"""
+    d = getattr(t, "device", None)
+    return None if d is None else (d.type, d.index)
+
+
 def kv_work_bytes(n_seq: int, n_pages: int) -> int:
     return lib().mi355x_kv_work_bytes(n_seq, n_pages)
 
@@ -270,6 +276,8 @@ def kv_cache(k, v, table, length, ref, status, work) -> KvCache:
         raise ValueError("k and v: [page, head, key, dim] of one shape, type and layout, dims contiguous")
     if table.dim() != 2:
         raise ValueError("table: [sequence, page]")
+    if len({_device(t) for t in (k, v, table, length, ref, status, work)}) > 1:
+        raise ValueError("the arrays of a cache lie on one device")
     b, need = k.element_size(), kv_work_bytes(table.shape[0], k.shape[0])
     if work.numel() * work.element_size() < need or not work.is_contiguous():
         raise ValueError(f"work: {need} bytes wanted")
@@ -279,6 +287,7 @@ def kv_cache(k, v, table, length, ref, status, work) -> KvCache:
     c.nb_key, c.nb_head, c.nb_page = k.stride(2) * b, k.stride(1) * b, k.stride(0) * b
     c.table, c.len, c.ref = _ints(table, 0, "table"), _ints(length, c.n_seq, "length"), _ints(ref, c.n_pages, "ref")
     c.status, c.work = _ints(status, 1, "status"), work.data_ptr()
+    c.device = _device(k)
     return c
 
 
@@ -305,6 +314,7 @@ class Ctx:
         self.h = lib().mi355x_ctx_create(device)
         if not self.h:
             raise RuntimeError("mi355x_ctx_create failed: " + (lib().mi355x_last_error() or b"").decode())
+        self.device = device
 
     def sync(self):
         rc = lib().mi355x_ctx_synchronize(self.h)
@@ -321,31 +331,45 @@ class Ctx:
             self.h = None
 
     # ---- the paged cache: each returns a Call (arrays as in kv_cache(); lists int32 on the device) ----
+    def _here(self, *arrays):
+        """Kernels read what they are given as memory of the context's device: host arrays and those of another one are refused."""
+        for t in arrays:
+            d = None if t is None else t.__dict__.get("device") if isinstance(t, KvCache) else _device(t)
+            if d is not None and d != ("cuda", self.device):
+                raise ValueError(f"an array on {d[0]}{'' if d[1] is None else f':{d[1]}'}, where one on the context's device, {self.device}, is wanted")
+
     def kv_reset_call(self, cache: KvCache) -> Call:
+        self._here(cache)
         return Call(self, "mi355x_kv_reset", C.byref(cache), keep=cache)
 
     def kv_append_call(self, cache: KvCache, seq, cu, k, v) -> Call:
+        self._here(cache, seq, cu, k, v)
         n, tk, tv = seq.numel(), _rows(k), _rows(v)
         return Call(self, "mi355x_kv_append", C.byref(cache), n, _ints(seq, n, "seq"), _ints(cu, n + 1, "cu"), C.byref(tk), C.byref(tv), keep=(cache, seq, cu, k, v))
 
     def kv_truncate_call(self, cache: KvCache, seq, keep) -> Call:
+        self._here(cache, seq, keep)
         n = seq.numel()
         return Call(self, "mi355x_kv_truncate", C.byref(cache), n, _ints(seq, n, "seq"), _ints(keep, n, "keep"), keep=(cache, seq, keep))
 
     def kv_fork_call(self, cache: KvCache, src, dst) -> Call:
+        self._here(cache, src, dst)
         n = src.numel()
         return Call(self, "mi355x_kv_fork", C.byref(cache), n, _ints(src, n, "src"), _ints(dst, n, "dst"), keep=(cache, src, dst))
 
     def kv_compact_call(self, cache: KvCache, to: KvCache) -> Call:
+        self._here(cache, to)
         return Call(self, "mi355x_kv_compact", C.byref(cache), C.byref(to), keep=(cache, to))
 
     def attn_paged_call(self, cache: KvCache, q, out, seq=None, scale: float = 1.0, window: int = 0, max_len: int = 0, work=None) -> Call:
+        self._here(cache, q, out, seq, work)
         d = AttnPagedDesc()
         d.q, d.dst, d.seq, d.scale, d.window, d.max_len = _rows(q), _rows(out), _ints(seq, q.shape[0], "seq"), scale, window, max_len
         d.work, d.work_bytes = (work.data_ptr() or None, work.numel() * work.element_size()) if work is not None else (None, 0)
         return Call(self, "mi355x_attn_paged", C.byref(cache), C.byref(d), keep=(cache, d, q, out, seq, work))
 
     def attn_packed_call(self, q, out, cu_q, k=None, v=None, cu_k=None, cache=None, seq=None, scale: float = 1.0, causal: bool = True, window: int = 0, max_q: int = 0) -> Call:
+        self._here(q, out, cu_q, k, v, cu_k, cache, seq)
         d, n = AttnPackedDesc(), cu_q.numel() - 1
         d.q, d.dst, d.cu_q, d.n = _rows(q), _rows(out), _ints(cu_q, 1, "cu_q"), n
         if cache is not None:
