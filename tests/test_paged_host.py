@@ -168,6 +168,21 @@ def test_calls_refuse_arrays_that_are_not_on_the_contexts_device():
         ka.kv_cache(k, k.clone(), On(i(4, 4), "cuda:0"), i(4), i(8), i(1), torch.zeros(ka.kv_work_bytes(4, 8), dtype=torch.uint8))
 
 
+def test_a_call_of_a_closed_context_is_refused():
+    """a call keeps the context that it was made up for: after close() that is freed memory"""
+    ctx = object.__new__(ka.Ctx)
+    ctx.h, ctx.device = CTX, 0
+    call = ctx.kv_reset_call(cache())
+    reached = []
+    call.fn = lambda *args: reached.append(args) or 0
+    call()
+    assert len(reached) == 1
+    ctx.h = None                                                     # what close() leaves
+    with pytest.raises(RuntimeError, match="closed"):
+        call()
+    assert len(reached) == 1
+
+
 def test_ctypes_mirrors_of_the_paged_structs(tmp_path):
     import subprocess
     from conftest import ROOT

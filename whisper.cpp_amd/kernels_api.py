@@ -302,6 +302,8 @@ class Call:
         self.ctx, self.name, self.fn, self.args, self.keep = ctx, name, getattr(lib(), name), (ctx.h, *args), (args, keep)
 
     def __call__(self):
+        if not self.ctx.h:
+            raise RuntimeError(f"{self.name}: the context is closed")
         rc = self.fn(*self.args)
         if rc:
             self.ctx.check(rc, self.name)
