@@ -326,6 +326,8 @@ MI355X_API int mi355x_flash_attn_ext_exact(mi355x_ctx * ctx, const mi355x_tensor
  * j % page_size.  Pages without a holder are free; the calls below hand out the LOWEST free ones, in the order of their list, so that equal
  * states and lists give equal tables.  All of it is the caller's memory and stays where it is: the calls only launch kernels on the context's
  * stream (nothing is allocated, copied to the host or waited for), so they can be captured into a graph and replayed with new lists.
+ * That stream waits for no other: a program whose rows, lists or queries come from another stream, or whose next step there reads the results, does
+ * that work on mi355x_ctx_stream() too, or puts events between.
  *
  * What a call finds wrong with DEVICE values — a sequence >= n_seq, one named twice, offsets that fall or leave the rows, too few free pages, a
  * full table row — it reports in *status (OR of enum mi355x_kv_status, never cleared by a call) and then changes nothing of the cache.  Lists may

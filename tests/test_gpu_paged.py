@@ -728,6 +728,41 @@ def test_scores_near_the_lowest_number_of_all(gpu):
         assert float((out[0, 0].double() - want).abs().max()) <= tol
 
 
+def test_calls_among_the_programs_own_work_on_the_contexts_stream(gpu):
+    """projections that make the rows, the calls, and a product that reads the result, one after the other on ctx.stream with no wait between them"""
+    ctx, ka, torch = gpu
+    p, n, heads, dim = Pool(gpu, heads=2, dim=64, kind="f16"), 60, 2, 64
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x, w = torch.randn(n, 4096, generator=gen, device="cuda"), [torch.randn(4096, heads * dim, generator=gen, device="cuda") / 64 for _ in range(3)]
+    late, w_o = torch.randn(4096, 4096, generator=gen, device="cuda") / 64, torch.randn(heads * dim, 32, generator=gen, device="cuda")
+    rows, out = [torch.zeros(n, heads, dim, device="cuda") for _ in range(3)], torch.zeros(n, heads, dim, device="cuda")
+    seq, cu, keep = p.ints([1, 4]), p.ints([0, 25, n]), p.ints([0, 0])
+    calls = [ctx.kv_truncate_call(p.c, seq, keep), ctx.kv_append_call(p.c, seq, cu, rows[1], rows[2]), ctx.attn_packed_call(rows[0], out, cu, cache=p.c, seq=seq, scale=0.125)]
+
+    def step(wait):
+        y = x
+        for _ in range(20):                                          # milliseconds before the rows are there
+            y = torch.mm(y, late)
+        for r, m in zip(rows, w):
+            torch.mm(y, m, out=r.view(n, heads * dim))
+        wait()
+        for call in calls:
+            call()
+        wait()
+        return torch.mm(out.view(n, heads * dim), w_o)
+
+    want = step(torch.cuda.synchronize)
+    for r in rows:
+        r.zero_()
+    out.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream)):
+        got = [step(lambda: None) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert want.abs().max() > 0 and all(torch.equal(g, want) for g in got)
+    p.status.zero_()
+
+
 def test_a_decode_loop_captured_into_a_graph_and_replayed(gpu):
     """append, attention, fork and truncate of a step captured once on the context's stream; every replay, with new lists and eager work of the program
     between the replays, equals the same step run eagerly on a second cache"""

@@ -323,6 +323,12 @@ class Ctx:
         if rc:
             raise RuntimeError(f"sync failed rc={rc}: {lib().mi355x_last_error().decode()}")
 
+    @property
+    def stream(self) -> int:
+        """The stream (hipStream_t) that every call is launched on.  It waits for no other, torch's among them: work on the same arrays belongs on it too
+        (torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream))), or events between the two."""
+        return lib().mi355x_ctx_stream(self.h)
+
     def check(self, rc: int, what: str = "op"):
         if rc != 0:
             raise RuntimeError(f"{what} failed rc={rc}: {(lib().mi355x_last_error() or b'').decode()}")
@@ -332,7 +338,7 @@ class Ctx:
             lib().mi355x_ctx_destroy(self.h)
             self.h = None
 
-    # ---- the paged cache: each returns a Call (arrays as in kv_cache(); lists int32 on the device) ----
+    # ---- the paged cache: each returns a Call (arrays as in kv_cache(); lists int32 on the device), made on this context's `stream` ----
     def _here(self, *arrays):
         """Kernels read what they are given as memory of the context's device: host arrays and those of another one are refused."""
         for t in arrays:
