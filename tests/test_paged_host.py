@@ -105,6 +105,14 @@ def test_attention_of_packed_rows_refuses_what_it_cannot_do():
     refused("mi355x_attn_packed", None)
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_attention_of_packed_rows_refuses_a_scale_that_is_no_number(scale):
+    """(a NaN came out as equal weights)"""
+    d = ka.AttnPackedDesc()
+    d.q, d.k, d.v, d.dst, d.cu_q, d.n, d.scale = rows(), rows(kind=ka.F16), rows(kind=ka.F16), rows(), AT, 1, scale
+    refused("mi355x_attn_packed", C.byref(d))
+
+
 def test_python_descriptions_refuse_arrays_that_do_not_fit():
     import torch
     k = torch.zeros(8, 2, 16, 64, dtype=torch.float16)

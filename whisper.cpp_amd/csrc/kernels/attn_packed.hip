@@ -437,7 +437,7 @@ extern "C" int mi355x_attn_packed(mi355x_ctx * ctx, const mi355x_attn_packed_des
     const int64_t H = d->q.ne[1], rows = d->q.ne[2];
     if (H < 1 || H % Hkv || H / Hkv > 128) return kv_refuse("attn_packed: the query heads are no multiple (up to 128) of the K/V heads");
     if (!kv_rows_ok(&d->q, dim, H) || !kv_rows_ok(&d->dst, dim, H) || d->dst.ne[2] != rows) return kv_refuse("attn_packed: q and dst are [head_dim, n_head, rows], F32 / F16 / BF16, 16-byte aligned");
-    if (d->n < 0 || d->window < 0 || d->max_q < 0) return kv_refuse("attn_packed: n, window or max_q");
+    if (d->n < 0 || d->window < 0 || d->max_q < 0 || !isfinite(d->scale)) return kv_refuse("attn_packed: n, window, max_q or scale");
     if (d->n == 0 || rows == 0) return 0;
     if (!d->cu_q || ((uintptr_t) d->cu_q | (uintptr_t) d->cu_k | (uintptr_t) d->seq) % 4) return kv_refuse("attn_packed: cu_q, cu_k or seq");
     const device_scope scope(ctx);
