@@ -329,9 +329,12 @@ MI355X_API int mi355x_flash_attn_ext_exact(mi355x_ctx * ctx, const mi355x_tensor
  * That stream waits for no other: a program whose rows, lists or queries come from another stream, or whose next step there reads the results, does
  * that work on mi355x_ctx_stream() too, or puts events between.
  *
- * What a call finds wrong with DEVICE values — a sequence >= n_seq, one named twice, offsets that fall or leave the rows, too few free pages, a
- * full table row — it reports in *status (OR of enum mi355x_kv_status, never cleared by a call) and then changes nothing of the cache.  Lists may
- * hold -1 for an entry to be left out (a padded batch).  Calls that change one cache follow one another (one stream, or ordered by events). */
+ * What a call that changes a cache finds wrong with DEVICE values — a sequence >= n_seq, one named twice, offsets that fall or leave the rows, too few
+ * free pages, a full table row — it reports in *status (OR of enum mi355x_kv_status, never cleared by a call) and then changes nothing of the cache
+ * (mi355x_kv_truncate leaves out the entry alone).  The attentions report page numbers outside the pool in *status, and nothing else: to them a
+ * sequence outside 0 .. n_seq-1 holds no keys, a length outside 0 .. max_pages * page_size is the nearer end, keys whose offsets fall or leave the rows
+ * are none, and of rows whose cu_q falls or leaves the rows it is not said which are written (no others are).  Lists may hold -1 for an entry to be
+ * left out (a padded batch).  Calls that change one cache follow one another (one stream, or ordered by events). */
 enum mi355x_kv_status {
     MI355X_KV_BAD_ARG      = 1,    /* a list entry, offset, length or table entry out of range, or a sequence named twice */
     MI355X_KV_ROW_FULL     = 2,    /* a sequence would need more than max_pages pages */
@@ -392,6 +395,8 @@ typedef struct mi355x_attn_paged_desc {
     void *          work;
     size_t          work_bytes;
 } mi355x_attn_paged_desc;
+/* for a call with exactly this n and max_len: whether the keys are split depends on both, so that fewer queries can need MORE (64 queries of 2048
+ * keys, 8 heads of 64: none; 63: 268484 bytes).  One area for several shapes is as large as the largest of their answers. */
 MI355X_API size_t mi355x_attn_paged_work_bytes(const mi355x_kv_cache * c, int n, int n_head, int max_len);
 MI355X_API int    mi355x_attn_paged(mi355x_ctx * ctx, const mi355x_kv_cache * c, const mi355x_attn_paged_desc * d);
 

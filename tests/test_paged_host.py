@@ -91,6 +91,20 @@ def test_attention_of_one_token_refuses_what_it_cannot_do():
     assert ka.kv_work_bytes(4, 8) > 0 and ka.kv_work_bytes(0, 8) == 0 and ka.kv_work_bytes(4, -1) == 0
 
 
+def test_the_work_area_is_for_one_shape_and_the_largest_answer_does_for_all():
+    """what the header says of its size: not monotone in the queries; an area that is a byte short of its own shape's is refused"""
+    c = cache(n_head_kv=8, max_pages=128, n_seq=256, nb_page=16384)
+    need = {n: ka.attn_paged_work_bytes(c, n, 8, 2048) for n in (1, 63, 64, 128)}
+    assert need[63] == 268484 > need[1] > 0 and need[64] == need[128] == 0
+    sizes = [ka.attn_paged_work_bytes(c, n, 8, 2048) for n in range(1, 129)]
+    d = ka.AttnPagedDesc()
+    d.scale, d.max_len, d.work = 1.0, 2048, AT
+    for n in (1, 2, 62, 63):
+        d.q, d.dst, d.work_bytes = rows(n, 8), rows(n, 8), sizes[n - 1] - 1
+        refused("mi355x_attn_paged", C.byref(c), C.byref(d))
+    assert max(sizes) == sizes[62]
+
+
 def test_attention_of_packed_rows_refuses_what_it_cannot_do():
     kv = rows(kind=ka.F16)
     for change in (dict(q=rows(heads=3)), dict(q=rows(dim=128)), dict(q=rows(heads=258)), dict(dst=rows(4)), dict(k=rows()), dict(v=rows(kind=ka.BF16)), dict(v=rows(2, kind=ka.F16)), dict(k=rows(dim=80, kind=ka.F16)),

@@ -292,6 +292,7 @@ def kv_cache(k, v, table, length, ref, status, work) -> KvCache:
 
 
 def attn_paged_work_bytes(cache: KvCache, n: int, n_head: int, max_len: int = 0) -> int:
+    """for a call of exactly this shape; an area for several shapes is as large as the largest of their answers (fewer queries can need more)"""
     return lib().mi355x_attn_paged_work_bytes(C.byref(cache), n, n_head, max_len)
 
 
