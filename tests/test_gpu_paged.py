@@ -763,6 +763,50 @@ def test_calls_among_the_programs_own_work_on_the_contexts_stream(gpu):
     p.status.zero_()
 
 
+@pytest.mark.parametrize("n,rows,max_q", [(1, 5, 8), (3, 5, 8), (100, 2, 4), (1, 90, 0), (3, 90, 0), (100, 70, 0)])
+@pytest.mark.parametrize("dim,heads", [(64, 2), (128, 4)])
+@pytest.mark.parametrize("before", [1, 40, 700])
+def test_rows_before_the_first_sequence(gpu, n, rows, max_q, dim, heads, before):
+    """offsets that do not begin at 0: the rows before them belong to no sequence, are left as they are, and nothing else changes"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=n, n_pages=n * 20, max_pages=20, page=16, heads=1, dim=dim, kind="f16")
+    lens = [300 + i % 7 for i in range(n)]
+    step = -(-n // 25)
+    for i in range(0, n, step):
+        assert p.append([(s, lens[s]) for s in range(i, min(i + step, n))], "f16") == 0
+    q = torch.randn(n * rows, heads, dim, generator=p.gen, device="cuda").half()
+    late = torch.cat([torch.full((before, heads, dim), float("nan"), device="cuda").half(), q])
+    cu, cu_late = [i * rows for i in range(n + 1)], [before + i * rows for i in range(n + 1)]
+    kv = torch.randn(before + n * rows, 1, dim, generator=p.gen, device="cuda").half()
+    for own in (False, True):
+        out, out_late = torch.full_like(q, 7.0), torch.full_like(late, 7.0)
+        on, on_late = (dict(k=kv[before:], v=kv[before:]), dict(k=kv, v=kv)) if own else (dict(cache=p.c), dict(cache=p.c))
+        p.run(ctx.attn_packed_call(q, out, p.ints(cu), scale=0.1, max_q=max_q, **on))
+        p.run(ctx.attn_packed_call(late, out_late, p.ints(cu_late), scale=0.1, max_q=max_q, **on_late))
+        assert (out_late[:before] == 7.0).all()
+        # the choice of a kernel goes by the rows of the call: both are within the bounds of the file's head of the same result
+        pool = kv if own else p.k[p.ref > 0].nan_to_num(0.0)
+        e = (dim + 8) * U["f32"] * 0.1 * float(q.float().abs().sum(2).max() * pool.float().abs().max())
+        per = math.expm1(4 * e) + 2 * U["f16"] + (max(rows, 306) + 32) * U["f32"]
+        size = float(kv.float().abs().max() if own else p.v[p.ref > 0].float().nan_to_num(0.0).abs().max())
+        assert bool(((out_late[before:].float() - out.float()).abs() <= 2 * (per * size + U["f16"] * out.float().abs())).all())
+
+
+@pytest.mark.parametrize("before,counts", [(3, [2, 0, 1]), (300, [200, 5, 0]), (5000, [1, 0, 600])])
+def test_rows_before_the_first_entry_of_an_append(gpu, before, counts):
+    ctx, ka, torch = gpu
+    a, b = (Pool(gpu, n_seq=3, n_pages=80, max_pages=60, page=16, heads=2, dim=64, kind="f16") for _ in range(2))
+    k, v = (torch.randn(before + sum(counts), 2, 64, generator=a.gen, device="cuda") for _ in range(2))
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    a.run(ctx.kv_append_call(a.c, a.ints([2, 0, 1]), a.ints(cu.tolist()), k[before:], v[before:]))
+    b.run(ctx.kv_append_call(b.c, b.ints([2, 0, 1]), b.ints((cu + before).tolist()), k, v))
+    for x in ("table", "len", "ref", "status"):
+        assert torch.equal(getattr(a, x), getattr(b, x)), x
+    assert a.len.tolist() == [counts[1], counts[2], counts[0]] and int(a.status) == 0
+    for x in ("k", "v"):                                             # (memory that nothing was written to is NaN)
+        assert torch.equal(getattr(a, x).nan_to_num(9.0), getattr(b, x).nan_to_num(9.0)), x
+
+
 def test_a_decode_loop_captured_into_a_graph_and_replayed(gpu):
     """append, attention, fork and truncate of a step captured once on the context's stream; every replay, with new lists and eager work of the program
     between the replays, equals the same step run eagerly on a second cache"""

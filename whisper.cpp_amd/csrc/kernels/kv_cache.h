@@ -136,7 +136,7 @@ template <typename A> __device__ __forceinline__ bool packed_find(const A & a, i
     for (; step > 0; step /= 64) {
         const int i = (int) min((int64_t) lo + (int64_t) lane * step, (int64_t) a.n);
         const unsigned long long m = __ballot(i < a.n && a.cu_q[i] / a.qt + i <= slot);
-        lo += max(__popcll(m) - 1, 0) * step;
+        lo += max((int) __popcll(m) - 1, 0) * step;                  // (a count is unsigned: no sequence begins at or before the slot, 0 - 1)
     }
     j.i = lo;
     j.r0 = a.cu_q[lo]; const int r1 = a.cu_q[lo + 1];

@@ -44,7 +44,7 @@ __device__ __forceinline__ int last_at_most_wave(const int * at, int n, int x) {
     while (step * 64 < n) step *= 64;
     for (; step > 0; step /= 64) {
         const int i = (int) min((int64_t) lo + (int64_t) lane * step, (int64_t) n - 1);
-        lo = min(lo + max(__popcll(__ballot(lo + (int64_t) lane * step < n && at[i] <= x)) - 1, 0) * step, n - 1);
+        lo = min(lo + max((int) __popcll(__ballot(lo + (int64_t) lane * step < n && at[i] <= x)) - 1, 0) * step, n - 1);
     }
     return lo;
 }
