@@ -807,6 +807,32 @@ def test_rows_before_the_first_entry_of_an_append(gpu, before, counts):
         assert torch.equal(getattr(a, x).nan_to_num(9.0), getattr(b, x).nan_to_num(9.0)), x
 
 
+@pytest.mark.parametrize("max_q,rows", [(0, 5), (8, 5), (0, 90)])
+def test_what_the_attentions_make_of_lists_and_lengths_out_of_range(gpu, max_q, rows):
+    """a sequence that is none holds no keys, a length beyond the row is the row's end, offsets that fall or leave the rows write nothing outside them; no status"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=3, n_pages=70, max_pages=20, page=16, heads=1, dim=64, kind="f16")
+    assert p.append([(0, 320), (1, 100)], "f16") == 0
+    q = torch.randn(6 * rows + 4, 2, 64, generator=p.gen, device="cuda").half()
+    full = lambda: torch.full((6 * rows + 4, 2, 64), 7.0, device="cuda")  # noqa: E731
+    packed = lambda out, cu, seq: p.run(ctx.attn_packed_call(q, out, p.ints(cu), cache=p.c, seq=p.ints(seq), scale=0.1, max_q=max_q))  # noqa: E731
+    cu = [i * rows for i in range(7)]
+    want, out, one, one_out = full(), full(), full()[:6], full()[:6]
+    paged = lambda to, seq: p.run(ctx.attn_paged_call(p.c, q[:6], to, seq=p.ints(seq), scale=0.1))  # noqa: E731
+    packed(want, cu, [0, 2, 0, 2, 1, 2])
+    paged(one, [0, 2, 0, 2, 1, 2])
+    assert (want[rows : 2 * rows] == 0).all()                        # sequence 2 is empty
+    p.len[0], p.len[2] = 2 ** 31 - 1, -5
+    packed(out, cu, [0, 3, 0, -9, 1, 2])                             # (in 0 the row is full: 320 keys)
+    paged(one_out, [0, 3, 0, -9, 1, 2])
+    assert torch.equal(out, want) and torch.equal(one_out, one)
+    for wrong in ([0, rows, 2 * rows, rows, 4 * rows, 5 * rows, 6 * rows], [-3, rows, 2 * rows, 3 * rows, 4 * rows, 5 * rows, 6 * rows], cu[:-1] + [2 ** 31 - 1], [5 * rows] * 3 + [0] * 4):
+        out = full()
+        packed(out, wrong, [0, 1, 0, 1, 0, 1])
+        assert (out[6 * rows :] == 7).all()
+    assert int(p.status) == 0
+
+
 def test_a_decode_loop_captured_into_a_graph_and_replayed(gpu):
     """append, attention, fork and truncate of a step captured once on the context's stream; every replay, with new lists and eager work of the program
     between the replays, equals the same step run eagerly on a second cache"""
