@@ -833,6 +833,118 @@ def test_what_the_attentions_make_of_lists_and_lengths_out_of_range(gpu, max_q, 
     assert int(p.status) == 0
 
 
+def expect_rows(torch, q, k, v, see, scale, kind, out_kind, round_q):
+    """expect() for rows q [R, H, D] at once, on the GPU in 64 bits; see [R, L].  Values that are not finite are counted apart: what a row does not see is not in its result"""
+    (R, H, D), (L, Hkv) = q.shape, k.shape[:2]
+    G = H // Hkv
+    q, k, v = (x.double().permute(1, 0, 2).contiguous() for x in (q, k, v))          # [heads, rows, D]
+    q = q.reshape(Hkv, G * R, D)                                     # head h is G h' + g: rows (g, r) of K/V head h'
+    seen = see.repeat(G, 1)
+    kt = k.transpose(1, 2).contiguous()
+    x = torch.where(seen, torch.matmul(q, kt) * scale, -math.inf)
+    w = torch.where(seen, torch.softmax(x, 2), 0.0) if L else x
+    w = torch.where(seen.any(1)[:, None], w, 0.0)
+    o = torch.matmul(w, v.nan_to_num(0.0, 0.0, 0.0))
+    size = torch.where(seen, torch.matmul(q.abs(), kt.abs()) * abs(scale), 0.0).amax(2) if L else torch.zeros(Hkv, G * R, device=q.device).double()
+    e = size * ((D + 8) * U["f32"] + (U[kind] if round_q else 0.0))
+    per = torch.expm1(4 * e) + 2 * U[kind] + (L + 32) * U["f32"]
+    top = v.nan_to_num(0.0, 0.0, 0.0).abs().amax((1, 2)) if L else torch.zeros(Hkv, device=q.device).double()
+    tol = (per * top[:, None])[..., None] + U[out_kind] * o.abs() + 1e-30
+    has = [torch.matmul(seen.double(), f(v).double()) > 0 for f in (torch.isposinf, torch.isneginf, torch.isnan)]
+    o = torch.where(has[0], math.inf, o)
+    o = torch.where(has[1], -math.inf, o)
+    o = torch.where(has[2] | (has[0] & has[1]), math.nan, o)
+    back = lambda y: y.reshape(H, R, D).permute(1, 0, 2)  # noqa: E731
+    return back(o), back(tol)
+
+
+# of each form of the packed attention: dims, K/V heads, heads, rows and keys of the sequences (None: as many), the caller's bound of the rows
+FORMS = {
+    "k_attn_paged 64": (64, 2, 4, [5, 8, 0, 1], [700, 300, 40, 290], 8),
+    "k_attn_paged 128": (128, 1, 5, [7, 1, 3], [800, 3, 420], 8),
+    "4, 1 64": (64, 2, 6, [50, 0, 3, 60], None, 0),
+    "4, 1 64 many": (64, 1, 32, [1500, 2501, 33, 100], None, 0),
+    "4, 2 64": (64, 2, 2, [300, 129, 1], [420, 129, 500], 0),
+    "4, 1 128": (128, 2, 6, [100, 0, 3, 77], None, 0),
+    "4, 1 128 many": (128, 4, 32, [700, 513, 1, 768, 200], None, 0),
+    "4, 2 128": (128, 3, 3, [40, 64, 3], [300, 700, 64], 0),
+    "8, 2 128": (128, 2, 4, [200, 131, 66], [500, 777, 66], 0),
+    "8, 1 128": (128, 8, 32, [1301, 0, 835], [1301, 40, 1500], 0),
+}
+
+
+@pytest.mark.parametrize("name", FORMS)
+@pytest.mark.parametrize("page,order", [(0, "head"), (0, "key"), (16, "key"), (64, "head")])
+@pytest.mark.parametrize("kind,io,causal,window,spoiled", [("f16", "f16", True, 0, False), ("bf16", "bf16", True, 0, True), ("f16", "f32", True, 333, True), ("bf16", "f32", False, 0, False), ("f16", "f16", False, 150, True),
+                                                           ("bf16", "bf16", True, 64, False)])
+def test_every_form_of_the_packed_attention(gpu, name, page, order, kind, io, causal, window, spoiled):
+    """each row tile and split of the waves that a call can get, by its name in the profile, with every kind of mask, infinities in tiles seen whole and in part, strided rows"""
+    ctx, ka, torch = gpu
+    dim, kv_heads, heads, q_lens, k_lens, max_q = FORMS[name]
+    n, ks, rng = len(q_lens), k_lens or q_lens, random.Random(1)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    cu, ck = (np.concatenate([[0], np.cumsum(x)]).tolist() for x in (q_lens, ks))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.randn(cu[-1] + 2, heads, dim, generator=gen, device="cuda").mul_(2).to(dt(torch, io))
+    out = torch.full((cu[-1] + 2, heads, dim), 7.0, device="cuda").to(dt(torch, io))
+    kv = [torch.randn(ck[-1], kv_heads, dim, generator=gen, device="cuda").to(dt(torch, kind)) for _ in range(2)]
+    if spoiled:
+        for i in range(n):
+            for j, d, x in ((ks[i] - 1, 1, math.inf), (ks[i] // 2, 2, -math.inf), (ks[i] // 3, 3, math.nan), (ks[i] // 2 + 1, 4, math.inf), (ks[i] - 2, 4, -math.inf), (0, 5, math.inf)):
+                if 0 <= j < ks[i]:
+                    kv[1][ck[i] + j, :, d] = x
+    args = dict(scale=dim ** -0.5, causal=causal, window=window, max_q=max_q)
+    if page:
+        held = [-(-x // page) for x in ks]
+        table, spread = torch.full((n + 1, max(held)), -1, dtype=torch.int32), rng.sample(range(sum(held) + 3), sum(held))
+        seq = rng.sample(range(n + 1), n)
+        shape = (sum(held) + 3, kv_heads, page, dim) if order == "head" else (sum(held) + 3, page, kv_heads, dim)
+        pools = [torch.full(shape, math.nan, device="cuda").to(dt(torch, kind)) for _ in range(2)]
+        pools = pools if order == "head" else [x.transpose(1, 2) for x in pools]
+        length, at = torch.zeros(n + 1, dtype=torch.int32), 0
+        for i in range(n):
+            pages = spread[at : at + held[i]]
+            at += held[i]
+            table[seq[i], : held[i]] = torch.tensor(pages, dtype=torch.int32)
+            length[seq[i]] = ks[i]
+            where = torch.arange(ks[i])
+            for pool, rows in zip(pools, kv):
+                pool[torch.tensor(pages, dtype=torch.long)[where // page].cuda(), :, (where % page).cuda()] = rows[ck[i] : ck[i + 1]]
+        zero = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+        status, dtab, dlen, ref, work = zero(1), table.cuda(), length.cuda(), zero(sum(held) + 3), torch.empty(ka.kv_work_bytes(n + 1, sum(held) + 3), dtype=torch.uint8, device="cuda")
+        c = ka.kv_cache(*pools, dtab, dlen, ref, status, work)
+        call = ctx.attn_packed_call(q, out, ints(cu), cache=c, seq=ints(seq), **args)
+    else:
+        wide = [torch.full((ck[-1] + 1, kv_heads, 2 * dim if order == "key" else dim), math.nan, device="cuda").to(dt(torch, kind)) for _ in range(2)]
+        for x, rows in zip(wide, kv):
+            x[: ck[-1], :, :dim] = rows
+        call = ctx.attn_packed_call(q, out, ints(cu), k=wide[0][..., :dim], v=wide[1][..., :dim], cu_k=ints(ck) if k_lens else None, **args)
+    torch.cuda.synchronize()
+    ctx.prof_reset()
+    ctx.prof(True)
+    call()
+    ctx.sync()
+    ran = [r["name"] for r in ctx.prof_report()]
+    ctx.prof(False)
+    ctx.prof_reset()
+    form = f"k_attn_packed<{kind}_ops, {dim}, {str(page > 0).lower()}, {name[:4]}>" if max_q == 0 else f"k_attn_paged<{kind}_ops, {dim}, 1, {0 if page == 16 else 1 if page else 2}, true>"
+    assert len(ran) == 1 and form in ran[0], (form, ran)
+    assert (out[cu[-1] :] == 7.0).all() and (not page or int(status) == 0)
+    for i in range(n):
+        Q, L = q_lens[i], ks[i]
+        if Q == 0:
+            continue
+        r = sorted(set(range(min(Q, 6))) | set(range(max(Q - 6, 0), Q)) | set(rng.sample(range(Q), min(Q, 40))))
+        j, own = torch.arange(L, device="cuda"), torch.tensor(r, device="cuda")[:, None] + L - Q
+        see = j <= own if causal else (j >= 0).expand(len(r), L)
+        see = see & (j > own - window) if window else see
+        o, tol = expect_rows(torch, q[[cu[i] + x for x in r]], kv[0][ck[i] : ck[i + 1]], kv[1][ck[i] : ck[i + 1]], see, dim ** -0.5, kind, io, io != kind)
+        try:
+            same(torch, out[[cu[i] + x for x in r]], o.cpu(), tol.cpu())
+        except AssertionError as e:
+            raise AssertionError(f"sequence {i} of {Q} rows and {L} keys: {e}")
+
+
 def test_a_decode_loop_captured_into_a_graph_and_replayed(gpu):
     """append, attention, fork and truncate of a step captured once on the context's stream; every replay, with new lists and eager work of the program
     between the replays, equals the same step run eagerly on a second cache"""
@@ -920,3 +1032,60 @@ def test_serving_streams_from_prompt_to_beams(gpu, kind, dim, kv_heads, heads, p
             p = other
             p.check(contents=False)
     p.check(contents=False)
+
+
+@pytest.mark.parametrize("n,n_seq,width", [(3000, 4000, 13), (8192, 20000, 7), (8192, 8192, 3), (1, 3, 20)])
+def test_forks_of_long_lists(gpu, n, n_seq, width):
+    """lists whose workgroups need more than 64 KB, or hold fewer columns at a time, against a restatement of tables"""
+    ctx, ka, torch = gpu
+    gen, rng = torch.Generator().manual_seed(n), random.Random(n)
+    n_pages = 500
+    lens = torch.randint(0, width * 4 + 1, (n_seq,), generator=gen, dtype=torch.int32)
+    column = torch.arange(width)
+    table = torch.where(column < (lens[:, None] + 3) // 4, torch.randint(0, n_pages, (n_seq, width), generator=gen), -1).int()
+    count = lambda t: torch.bincount(t[t >= 0].long(), minlength=n_pages).int()  # noqa: E731
+    k = torch.zeros(n_pages, 1, 4, 64, dtype=torch.float16, device="cuda")
+    dtab, dlen, ref, status, work = table.cuda(), lens.cuda(), count(table).cuda(), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.empty(ka.kv_work_bytes(n_seq, n_pages), dtype=torch.uint8, device="cuda")
+    c = ka.kv_cache(k, k.clone(), dtab, dlen, ref, status, work)
+    dst = rng.sample(range(n_seq), n)
+    src = [rng.randrange(-1, n_seq) for _ in range(n)]
+    for i in range(0, n, 5):
+        dst[i] = -1 if i % 2 else dst[i]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    dsrc, ddst = ints(src), ints(dst)
+    torch.cuda.synchronize()
+    ctx.kv_fork_call(c, dsrc, ddst)()
+    ctx.sync()
+    new, new_len = table.clone(), lens.clone()
+    for a, b in zip(src, dst):
+        if b >= 0:
+            new[b], new_len[b] = (table[a], lens[a]) if a >= 0 else (torch.full((width,), -1, dtype=torch.int32), 0)
+    assert torch.equal(dtab.cpu(), new) and torch.equal(dlen.cpu(), new_len) and torch.equal(ref.cpu(), count(new)) and int(status) == 0
+    if n > 1:                                                        # the last entry once more the first's row: nothing changes
+        ddst[0], ddst[-1] = 7, 7
+        torch.cuda.synchronize()
+        ctx.kv_fork_call(c, dsrc, ddst)()
+        ctx.sync()
+        assert torch.equal(dtab.cpu(), new) and torch.equal(dlen.cpu(), new_len) and torch.equal(ref.cpu(), count(new)) and int(status) == ka.KV_BAD_ARG
+
+
+@pytest.mark.parametrize("heads,dim,kind,io,counts", [(64, 128, "bf16", "f32", [3, 1, 700, 20]), (256, 128, "f16", "bf16", [33, 0, 2]), (1, 64, "f16", "f16", [4000, 1, 999, 17]), (5, 64, "bf16", "bf16", [1500, 3000])])
+def test_appends_of_wide_rows_and_of_many(gpu, heads, dim, kind, io, counts):
+    """rows of more pieces than a workgroup loads at once, and as many narrow rows to a workgroup as it takes"""
+    ctx, ka, torch = gpu
+    page, n = 16, len(counts)
+    held = [-(-x // page) for x in counts]
+    p = Pool(gpu, n_seq=n, n_pages=sum(held) + 1, max_pages=max(held), page=page, heads=heads, dim=dim, kind=kind)
+    k, v = (torch.randn(sum(counts) + 2, heads, dim, generator=p.gen, device="cuda").to(dt(torch, io)) for _ in range(2))
+    cu = np.concatenate([[0], np.cumsum(counts)]).tolist()
+    p.run(ctx.kv_append_call(p.c, p.ints(list(range(n))), p.ints(cu), k, v))
+    assert int(p.status) == 0 and p.len.tolist() == counts
+    table, taken = p.table.cpu(), 0
+    for i in range(n):                                               # free pages in ascending order, entry by entry
+        assert table[i].tolist() == list(range(taken, taken + held[i])) + [-1] * (max(held) - held[i])
+        for pool, rows in ((p.k, k), (p.v, v)):
+            got = pool[taken : taken + held[i]].transpose(1, 2).reshape(-1, heads, dim)
+            assert torch.equal(got[: counts[i]], rows[cu[i] : cu[i + 1]].to(dt(torch, kind)))
+            assert got[counts[i] :].isnan().all()
+        taken += held[i]
+    assert p.ref.tolist() == [1] * taken + [0] and p.k[taken:].isnan().all()
