@@ -266,3 +266,41 @@ def test_every_group_of_heads_finds_a_form_of_the_packed_attention():
     assert r.returncode == 0, (r.returncode, lines[-1:])
     name, *answers = lines[-1].split()
     assert name == "answers:" and answers and all(int(x) > 0 for x in answers), lines[-1]
+
+
+def test_a_build_compiles_every_kernel_source_when_told_to_and_after_a_change_of_flags(monkeypatch, tmp_path):
+    """nothing is run: the commands are"""
+    import os
+    from whisper_cpp_amd import build
+    ran = []
+    monkeypatch.setattr(build, "_run", lambda cmd: ran.append([str(x) for x in cmd]) or "")
+    monkeypatch.setattr(build, "LIB", tmp_path / "lib")
+    monkeypatch.setattr(build, "BUILD", tmp_path / "build")
+    compiled = lambda: sorted(os.path.basename(c[c.index("-c") + 1]) for c in ran if "-c" in c)  # noqa: E731
+    build.build_kernels()
+    assert compiled() == sorted(build.KERNEL_SRCS) and "-shared" in ran[-1]
+    now = max(f.stat().st_mtime for f in [build.Path(build.__file__), *(build.CSRC / "kernels").iterdir(), *(build.ROOT / "include").iterdir()]) + 5
+    made = [tmp_path / "build" / "kernels" / (s + ".o") for s in build.KERNEL_SRCS] + [tmp_path / "lib" / "libmi355x_kernels.so"]
+    for f in made:
+        f.write_bytes(b"")
+        os.utime(f, (now, now))
+    ran.clear()
+    build.build_kernels()
+    assert ran == []
+    build.build_kernels(force=True)
+    assert compiled() == sorted(build.KERNEL_SRCS) and "-shared" in ran[-1]
+    for f in made[:-1]:
+        f.unlink()
+    ran.clear()
+    build.build_kernels()                                            # the library alone, newer than all sources
+    assert ran == []
+    build.build_kernels(force=True)
+    assert compiled() == sorted(build.KERNEL_SRCS)
+    for f in made[:-1]:
+        f.write_bytes(b"")
+    flags = build.Path(build.__file__).stat().st_mtime
+    for f in made:
+        os.utime(f, (flags - 1, flags - 1))                          # objects older than the flags
+    ran.clear()
+    build.build_kernels()
+    assert compiled() == sorted(build.KERNEL_SRCS)

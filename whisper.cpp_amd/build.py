@@ -6,7 +6,7 @@
                                              oracle/_ref/libggml-base.so to link against.
   oracle/liboracle.so, oracle/_ref/*       : test infrastructure (see oracle/Makefile).
 
-hipcc cross-compiles for gfx950 without a GPU.  Objects are cached by source mtime under build/.
+hipcc cross-compiles for gfx950 without a GPU.  Objects are cached under build/ by the times of their sources, headers and this file.
 """
 import os
 import subprocess
@@ -50,19 +50,20 @@ def _stale(out: Path, deps):
     return any(Path(d).stat().st_mtime > t for d in deps if Path(d).exists())
 
 
-def build_kernels(verbose=False):
+def build_kernels(verbose=False, force=False):
+    """`force`: every source is compiled, whatever is there.  Otherwise those whose objects are older than they, their headers or this file (its flags)."""
     LIB.mkdir(exist_ok=True)
     (BUILD / "kernels").mkdir(parents=True, exist_ok=True)
-    hdrs = [CSRC / "kernels" / "common.h", CSRC / "kernels" / "decode_common.h", CSRC / "kernels" / "qrows.h", CSRC / "kernels" / "kv_cache.h", ROOT / "include" / "mi355x_kernels.h"]
+    hdrs = [CSRC / "kernels" / "common.h", CSRC / "kernels" / "decode_common.h", CSRC / "kernels" / "qrows.h", CSRC / "kernels" / "kv_cache.h", ROOT / "include" / "mi355x_kernels.h", Path(__file__)]
     so = LIB / "libmi355x_kernels.so"
-    if not _stale(so, [CSRC / "kernels" / s for s in KERNEL_SRCS] + hdrs) and not any((BUILD / "kernels").iterdir()):
+    if not force and not _stale(so, [CSRC / "kernels" / s for s in KERNEL_SRCS] + hdrs) and not any((BUILD / "kernels").iterdir()):
         return so                                        # a library that travelled without its objects and is newer than its sources
     objs, jobs = [], []
     for s in KERNEL_SRCS:
         src = CSRC / "kernels" / s
         obj = BUILD / "kernels" / (s + ".o")
         objs.append(obj)
-        if _stale(obj, [src] + hdrs):
+        if force or _stale(obj, [src] + hdrs):
             jobs.append([HIPCC, *HIPFLAGS, *EXTRA_FLAGS.get(s, []), "-c", str(src), "-o", str(obj)])
     with ThreadPoolExecutor(max_workers=8) as ex:
         for out in ex.map(_run, jobs):
@@ -120,8 +121,8 @@ def build_host():
     return so
 
 
-def build_all(verbose=False):
-    k = build_kernels(verbose)
+def build_all(verbose=False, force=False):
+    k = build_kernels(verbose, force)
     o = build_oracle()
     b = build_backend()
     build_host()
