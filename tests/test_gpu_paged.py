@@ -1089,3 +1089,149 @@ def test_appends_of_wide_rows_and_of_many(gpu, heads, dim, kind, io, counts):
             assert got[counts[i] :].isnan().all()
         taken += held[i]
     assert p.ref.tolist() == [1] * taken + [0] and p.k[taken:].isnan().all()
+
+
+@pytest.mark.parametrize("kind,dim,order", [("f16", 64, "head"), ("bf16", 128, "key")])
+def test_places_beyond_four_gigabytes(gpu, kind, dim, order):
+    """pages more than a gigabyte apart, rows of packed prompts too: every byte offset in 64 bits, in each call"""
+    ctx, ka, torch = gpu
+    page, heads, n_pages, apart = 16, 2, 7, (1 << 30) + 4096       # (elements of 2 bytes: 2 GiB and a bit)
+    inner = (page * dim, dim) if order == "head" else (dim, heads * dim)
+    whole = [torch.empty(apart * (n_pages - 1) + heads * page * dim, dtype=dt(torch, kind), device="cuda") for _ in range(2)]
+    k, v = (x.as_strided((n_pages, heads, page, dim), (apart, *inner, 1)) for x in whole)
+    zero = lambda *m: torch.zeros(*m, dtype=torch.int32, device="cuda")  # noqa: E731
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    work = torch.empty(ka.kv_work_bytes(2, n_pages), dtype=torch.uint8, device="cuda")
+    table, length, ref, status = zero(2, 5), zero(2), zero(n_pages), zero(1)
+    c = ka.kv_cache(k, v, table, length, ref, status, work)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rows = [torch.randn(75, heads, dim, generator=gen, device="cuda").to(dt(torch, kind)) for _ in range(2)]
+    q = torch.randn(8, 4, dim, generator=gen, device="cuda").to(dt(torch, kind))
+
+    def run(call):
+        torch.cuda.synchronize()
+        call()
+        ctx.sync()
+
+    def hold(out, i, last, first, keys):
+        o, tol = expect(torch, q[i].cpu(), *(x[first : first + keys].cpu() for x in rows), torch.arange(keys) <= last, 0.1, kind, kind, "f32", False, True)
+        same(torch, out[i], o, tol)
+
+    run(ctx.kv_reset_call(c))
+    run(ctx.kv_append_call(c, ints([1, 0]), ints([0, 5, 75]), *rows))            # sequence 1 in page 0, sequence 0 in pages 1 .. 5
+    assert int(status) == 0 and table.tolist() == [[1, 2, 3, 4, 5], [0, -1, -1, -1, -1]]
+    small = [torch.zeros(n_pages, heads, page, dim, dtype=dt(torch, kind), device="cuda") for _ in range(2)]
+    table2, length2, ref2, work2 = zero(2, 5), zero(2), zero(n_pages), torch.empty_like(work)
+    to = ka.kv_cache(*small, table2, length2, ref2, status, work2)
+    run(ctx.kv_reset_call(to))
+    run(ctx.kv_compact_call(c, to))                                  # from far apart to close together, and back
+    for x, y in zip((k, v), small):
+        for p, filled in ((0, 5), (1, 16), (3, 16), (5, 6)):
+            assert torch.equal(x[p, :, :filled], y[p, :, :filled])
+    for which in (c, to):
+        out = torch.zeros(2, 4, dim, device="cuda")
+        run(ctx.attn_paged_call(which, q[:2], out, scale=0.1))
+        hold(out, 0, 69, 5, 70)
+        hold(out, 1, 4, 0, 5)
+        for max_q in (0, 8):
+            out = torch.zeros(8, 4, dim, device="cuda")
+            run(ctx.attn_packed_call(q, out, ints([0, 6, 8]), cache=which, scale=0.1, max_q=max_q))
+            for i in range(6):
+                hold(out, i, 64 + i, 5, 70)
+            hold(out, 7, 4, 0, 5)
+    del whole, k, v, c, x
+    torch.cuda.empty_cache()
+    far = [torch.empty(300 * (1 << 24), dtype=dt(torch, kind), device="cuda").as_strided((300, heads, dim), (1 << 24, dim, 1)) for _ in range(2)]     # rows of a prompt 32 MiB apart
+    for i, x in enumerate(far):
+        x.copy_(torch.cat([rows[i], torch.randn(225, heads, dim, generator=gen, device="cuda").to(dt(torch, kind))]))
+    rows = [x.contiguous() for x in far]
+    for max_q in (0, 8):
+        out = torch.zeros(8, 4, dim, device="cuda")
+        run(ctx.attn_packed_call(q[:6], out[:6], ints([0, 6]), k=far[0], v=far[1], cu_k=ints([0, 300]), scale=0.1, max_q=max_q))
+        for i in range(6):
+            hold(out, i, 294 + i, 0, 300)
+    run(ctx.kv_reset_call(to))
+    run(ctx.kv_append_call(to, ints([1, 0]), ints([225, 230, 300]), *far))       # the last rows: 7 GiB from the first
+    assert int(status) == 0
+    assert torch.equal(small[0][1], rows[0][230:246].transpose(0, 1)) and torch.equal(small[1][5, :, :6], rows[1][294:300].transpose(0, 1))
+    del far
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("page,order", [(1, "head"), (2, "key"), (1024, "head"), (4096, "key")])
+@pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 128)])
+def test_the_smallest_and_the_largest_pages(gpu, page, order, kind, dim):
+    ctx, ka, torch = gpu
+    lens = [4500, 0, 1, 700, 1025]
+    need = sum(-(-x // page) for x in lens)
+    p = Pool(gpu, n_seq=5, n_pages=need + 5, max_pages=-(-4501 // page), page=page, heads=1, dim=dim, kind=kind, order=order)
+    assert p.append(list(enumerate(lens)), kind) == 0
+    p.fork([(0, 1)])
+    assert p.append([(1, 1), (3, 2)], kind) == 0
+    p.truncate([(0, 4097)])
+    lens = [len(x) for x in p.keys]
+    p.check(contents=False)
+    q = torch.randn(5 * 6, 4, dim, generator=p.gen, device="cuda").to(dt(torch, kind))
+    flat = [[torch.stack([x[w] for x in keys]) for w in (0, 1)] for keys in p.keys]
+    out, work = torch.zeros(5, 4, dim, device="cuda"), torch.empty(max(16, ka.attn_paged_work_bytes(p.c, 5, 4)), dtype=torch.uint8, device="cuda")
+    p.run(ctx.attn_paged_call(p.c, q[:5], out, scale=0.1, work=work))
+    for s in range(5):
+        o, tol = expect(torch, q[s].cpu(), *flat[s], torch.ones(lens[s], dtype=torch.bool), 0.1, kind, kind, "f32", False, True)
+        same(torch, out[s], o, tol)
+    for max_q in (0, 8):
+        out = torch.zeros(30, 4, dim, device="cuda")
+        p.run(ctx.attn_packed_call(q, out, p.ints([0, 6, 12, 18, 24, 30]), cache=p.c, scale=0.1, max_q=max_q))
+        for s in range(5):
+            for r in range(6):
+                o, tol = expect(torch, q[6 * s + r].cpu(), *flat[s], torch.arange(lens[s]) <= lens[s] - 6 + r, 0.1, kind, kind, "f32", False, True)
+                same(torch, out[6 * s + r], o, tol)
+    p.check()
+
+
+def test_prompts_and_a_compaction_captured_into_a_graph_and_replayed(gpu):
+    """reset, append, packed attention (the form of eight waves and the one for few rows) and compact in one graph, with new lists and rows between the replays"""
+    ctx, ka, torch = gpu
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    n, heads, kv_heads, dim, rows, keys = 3, 16, 2, 128, 2700, 2700
+    ends = [[0, 900, 1800, 2700], [0, 1, 2500, 2700], [0, 0, 2700, 2700], [0, 1300, 1300, 1999]]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    zero = lambda *m: torch.zeros(*m, dtype=torch.int32, device="cuda")  # noqa: E731
+    cu, few = ints(ends[0]), ints([0, 4, 8, 12])
+    q, k, v = torch.zeros(rows, heads, dim, device="cuda").half(), *(torch.zeros(keys, kv_heads, dim, device="cuda").half() for _ in range(2))
+    status, sets = zero(1), []
+    for _ in range(2):
+        cells = []
+        for _ in range(2):
+            pool = [torch.zeros(200, kv_heads, 16, dim, device="cuda").half() for _ in range(2)]
+            rest = [zero(n, 180), zero(n), zero(200), status, torch.empty(ka.kv_work_bytes(n, 200), dtype=torch.uint8, device="cuda")]
+            cells.append((ka.kv_cache(*pool, *rest), pool, rest))
+        outs = [torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q[:12])]
+        a, b = cells[0][0], cells[1][0]
+        seq = ints([2, 0, 1])
+        calls = [ctx.kv_reset_call(a), ctx.kv_append_call(a, seq, cu, k, v), ctx.attn_packed_call(q, outs[0], cu, k=k, v=v, scale=0.1, window=500), ctx.kv_reset_call(b), ctx.kv_compact_call(a, b),
+                 ctx.attn_packed_call(q, outs[1], cu, cache=b, seq=seq, scale=0.1, window=500), ctx.attn_packed_call(q[:12], outs[2], few, cache=b, seq=seq, scale=0.1, max_q=8)]
+        sets.append((calls, cells, outs))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for call in sets[1][0]:
+            call()
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    for rep in range(6):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        cu.copy_(ints(ends[rep % len(ends)]))
+        for _, cells, outs in sets:
+            for x in outs:
+                x.fill_(7.0)
+        torch.cuda.synchronize()
+        for call in sets[0][0]:
+            call()
+        ctx.sync()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(status) == 0
+        for x, y in zip(sets[0][2], sets[1][2]):
+            assert torch.equal(x, y), rep
+        for (_, pool, rest), (_, pool2, rest2) in zip(sets[0][1], sets[1][1]):
+            assert all(torch.equal(x, y) for x, y in zip(pool + rest[:3], pool2 + rest2[:3])), rep
