@@ -127,6 +127,25 @@ def test_attention_of_packed_rows_refuses_a_scale_that_is_no_number(scale):
     refused("mi355x_attn_packed", C.byref(d))
 
 
+def test_calls_of_more_threads_than_a_launch_has_are_refused_before_anything_is_launched():
+    c = cache()
+    refused("mi355x_kv_truncate", C.byref(c), 1 << 24, AT, AT)
+    many = rows(n=1 << 24, dim=64, kind=ka.F16)
+    refused("mi355x_kv_append", C.byref(c), 1, AT, AT, C.byref(many), C.byref(many))
+    refused("mi355x_kv_fork", C.byref(cache(page_size=1, nb_page=2048, max_pages=1 << 28)), 1, AT, AT)
+    other = dict(k=AT + 1024, v=AT + 2048, table=AT + 64, len=AT + 128, ref=AT + 192, work=AT + 256)
+    refused("mi355x_kv_compact", C.byref(cache(n_pages=1 << 27)), C.byref(cache(n_pages=1 << 27, **other)))
+    d = ka.AttnPagedDesc()
+    d.scale, d.max_len, d.seq = 1.0, 16, AT
+    d.q, d.dst = (rows(n=65535, heads=256) for _ in range(2))
+    refused("mi355x_attn_paged", C.byref(cache(max_pages=1)), C.byref(d))
+    d.q, d.dst = (rows(n=4096, heads=2048) for _ in range(2))
+    refused("mi355x_attn_paged", C.byref(cache(max_pages=1)), C.byref(d))
+    p = ka.AttnPackedDesc()
+    p.q, p.k, p.v, p.dst, p.cu_q, p.n, p.scale = rows(n=1 << 24, heads=256), rows(n=64, heads=256, kind=ka.F16), rows(n=64, heads=256, kind=ka.F16), rows(n=1 << 24, heads=256), AT, 1, 1.0
+    refused("mi355x_attn_packed", C.byref(p))
+
+
 def test_python_descriptions_refuse_arrays_that_do_not_fit():
     import torch
     k = torch.zeros(8, 2, 16, 64, dtype=torch.float16)

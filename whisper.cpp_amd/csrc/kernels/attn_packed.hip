@@ -382,7 +382,7 @@ static int launch_packed_as(mi355x_ctx * ctx, PackedArgs & a, int64_t Hkv) {
     a.qt = 32 * NW / KG / a.G;
     if (a.qt < 1) return kv_refuse("attn_packed: a group of more heads than a workgroup has rows");      // (launch_packed chooses a form that has them)
     const int64_t blocks = ((int64_t) a.rows_q / a.qt + a.n) * Hkv;
-    if (blocks > INT32_MAX) return kv_refuse("attn_packed: too many rows for one launch");
+    if (!kv_fits(blocks, 64 * NW)) return kv_refuse("attn_packed: too many rows for one launch");
     const uint32_t lds = (NW == 8 ? 3 * 3 * 64 : KG == 2 ? 3 * 64 : 3 * 32) * D * 2 + 16;
     const int rl = kv_allow_lds(ctx, (const void *) k_attn_packed<O, D, PAGED, NW, KG>, lds, allowed);
     if (rl) return rl;

@@ -486,7 +486,7 @@ static int launch_paged(mi355x_ctx * ctx, PagedArgs & a) {
 template <typename O, int D>
 static int launch_few(mi355x_ctx * ctx, PagedArgs & a, bool paged) {
     const int64_t blocks = ((int64_t) a.rows_q / a.qt + a.n) * a.c.Hkv * a.groups;
-    if (blocks > INT32_MAX) return kv_refuse("attn_packed: too many rows for one launch");
+    if (!kv_fits(blocks, 512)) return kv_refuse("attn_packed: too many rows for one launch");
     if (!paged) return launch_as<O, D, 1, ROWS, true>(ctx, a, blocks, 512);
     return a.c.shift >= 5 ? launch_as<O, D, 1, BIG_PAGES, true>(ctx, a, blocks, 512) : launch_as<O, D, 1, SMALL_PAGES, true>(ctx, a, blocks, 512);
 }
@@ -510,7 +510,7 @@ extern "C" int mi355x_attn_paged(mi355x_ctx * ctx, const mi355x_kv_cache * c, co
     const int64_t H = d->q.ne[1], n = d->q.ne[2];
     if (H < 1 || H > 32768 || H % c->n_head_kv) return kv_refuse("attn_paged: the query heads are no multiple of the K/V heads");
     if (!kv_rows_ok(&d->q, c->head_dim, H) || !kv_rows_ok(&d->dst, c->head_dim, H) || d->dst.ne[2] != n) return kv_refuse("attn_paged: q and dst are [head_dim, n_head, n], F32 / F16 / BF16, 16-byte aligned");
-    if (n > INT32_MAX / 32768 || n * H > INT32_MAX / 8) return kv_refuse("attn_paged: too many queries");
+    if (n > INT32_MAX / 32768 || !kv_fits(n * H, n > 4096 ? 512 : 1024)) return kv_refuse("attn_paged: too many queries");      // (a workgroup for each query and head at most; 1024 threads: k_attn_join)
     if (!d->seq && n > c->n_seq) return kv_refuse("attn_paged: more queries than sequences");
     if ((uintptr_t) d->seq % 4 || d->window < 0 || d->max_len < 0) return kv_refuse("attn_paged: seq, window or max_len");
     if (n == 0) return 0;

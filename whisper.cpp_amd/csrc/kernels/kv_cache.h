@@ -23,6 +23,9 @@ struct kvc {
 
 static inline int kv_refuse(const char * what) { mi355x_set_error("%s", what); return MI355X_E_UNSUPPORTED; }
 
+// a launch has at most 2^32 - 1 threads: looked at before the first launch of a call, so that none is done by half
+static inline bool kv_fits(int64_t blocks, int64_t threads) { return blocks <= UINT32_MAX / threads; }
+
 // argument checks of every call that takes a cache; fills `o`
 static inline int kv_view(const mi355x_kv_cache * c, kvc * o) {
     if (!c) return kv_refuse("kv cache: NULL");

@@ -317,6 +317,7 @@ extern "C" int mi355x_kv_append(mi355x_ctx * ctx, const mi355x_kv_cache * c, int
     if (n < 0 || n > c->n_seq) return kv_refuse("kv_append: more entries than sequences");
     if (n == 0) return 0;
     if (!seq || !cu || ((uintptr_t) seq | (uintptr_t) cu) % 4) return kv_refuse("kv_append: seq or cu");
+    if (!kv_fits(k->ne[2] + n, 256)) return kv_refuse("kv_append: too many rows for one launch");
     const device_scope scope(ctx);
     a.seq = seq; a.cu = cu; a.n = n; a.rows = (int) k->ne[2]; a.type_in = k->type; a.bf16 = c->type == MI355X_TYPE_BF16;
     a.k = (const char *) k->data; a.k_nb1 = k->nb[1]; a.k_nb2 = k->nb[2];
@@ -357,6 +358,7 @@ extern "C" int mi355x_kv_truncate(mi355x_ctx * ctx, const mi355x_kv_cache * c, i
     KvTruncateArgs a; const int rc = kv_view(c, &a.c);
     if (rc) return rc;
     if (!ctx || n < 0 || (n > 0 && (!seq || !keep || ((uintptr_t) seq | (uintptr_t) keep) % 4))) return kv_refuse("kv_truncate: arguments");
+    if (!kv_fits(n, 256)) return kv_refuse("kv_truncate: too many entries for one launch");
     const device_scope scope(ctx);
     a.seq = seq; a.keep = keep; a.n = n;
     return emit(ctx, "kv_truncate", k_kv_truncate, dim3((uint32_t) n), dim3(256), 0, a);
@@ -415,10 +417,12 @@ extern "C" int mi355x_kv_fork(mi355x_ctx * ctx, const mi355x_kv_cache * c, int n
     const size_t fixed = ((size_t) c->n_seq + 31) / 32 * 4 + (size_t) n * 4;
     while (a.cshift > 0 && fixed + ((size_t) n << a.cshift) * 4 > 128 * 1024) a.cshift--;
     const size_t lds = fixed + ((size_t) n << a.cshift) * 4;         // <= 128 KB
+    const int64_t blocks = ((int64_t) c->max_pages + (1 << a.cshift) - 1) >> a.cshift;
+    if (!kv_fits(blocks, 256)) return kv_refuse("kv_fork: the table is too wide for one launch");
     static std::atomic<uint64_t> allowed{0};
     const int rl = kv_allow_lds(ctx, (const void *) k_kv_fork, (uint32_t) lds, allowed);
     if (rl) return rl;
-    return emit(ctx, "kv_fork", k_kv_fork, dim3((uint32_t) ((c->max_pages + (1 << a.cshift) - 1) >> a.cshift)), dim3(256), (uint32_t) lds, a);
+    return emit(ctx, "kv_fork", k_kv_fork, dim3((uint32_t) blocks), dim3(256), (uint32_t) lds, a);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -552,7 +556,7 @@ extern "C" int mi355x_kv_compact(mi355x_ctx * ctx, const mi355x_kv_cache * from,
     a.table_blocks = (int) (tb > 1024 ? 1024 : tb);
     const int64_t pages = from->n_pages < to->n_pages ? from->n_pages : to->n_pages;     // at most so many are held and fit
     const int64_t blocks = a.table_blocks + pages * a.slices;
-    if (per > INT32_MAX || blocks > INT32_MAX) return kv_refuse("kv_compact: pools too large for one launch");
+    if (per > INT32_MAX || !kv_fits(blocks, 256)) return kv_refuse("kv_compact: pools too large for one launch");
     if (from->n_pages <= KV_SMALL_PAGES && pages * a.slices <= KV_SMALL_SLICES) {
         a.table_blocks = (int) (entries / 256 + 1 > 1024 ? 1024 : entries / 256 + 1);
         return emit(ctx, "kv_compact", k_kv_compact_small, dim3((uint32_t) (a.table_blocks + pages * a.slices)), dim3(256), 0, a);
