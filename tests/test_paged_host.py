@@ -160,6 +160,36 @@ def test_python_descriptions_refuse_arrays_that_do_not_fit():
             ka.kv_cache(**{**ok, **change})
 
 
+def test_a_cache_and_its_calls_hold_on_to_their_arrays():
+    """a work area made in the call itself, as the documents have it, is not given back while a call can still use it"""
+    import gc
+    import weakref
+    import torch
+    ctx = object.__new__(ka.Ctx)
+    ctx.h, ctx.device = CTX, 0
+    made = []
+
+    class On:
+        def __init__(self, t):
+            self.t, self.device = t, torch.device("cuda:0")          # (a host array that says it lies on the device: nothing is launched)
+            made.append(weakref.ref(self))
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    i = lambda *n: On(torch.zeros(*n, dtype=torch.int32))  # noqa: E731
+    pool = lambda: On(torch.zeros(8, 2, 16, 64, dtype=torch.float16))  # noqa: E731
+    c = lambda: ka.kv_cache(pool(), pool(), i(4, 4), i(4), i(8), i(1), On(torch.zeros(ka.kv_work_bytes(4, 8), dtype=torch.uint8)))  # noqa: E731
+    row = lambda: On(torch.zeros(3, 2, 64))  # noqa: E731
+    calls = [ctx.kv_reset_call(c()), ctx.kv_append_call(c(), i(2), i(3), row(), row()), ctx.kv_truncate_call(c(), i(2), i(2)), ctx.kv_fork_call(c(), i(2), i(2)), ctx.kv_compact_call(c(), c()),
+             ctx.attn_paged_call(c(), row(), row(), seq=i(3), work=On(torch.zeros(64, dtype=torch.uint8))), ctx.attn_packed_call(row(), row(), i(3), cache=c(), seq=i(2))]
+    gc.collect()
+    assert len(made) == 7 * 8 + 16 and all(m() is not None for m in made)
+    calls.clear()
+    gc.collect()
+    assert all(m() is None for m in made)
+
+
 def test_calls_refuse_arrays_that_are_not_on_the_contexts_device():
     """host memory, or another device's, is no memory for a kernel: refused where the call is made up, before there is anything to launch"""
     import torch

@@ -271,7 +271,7 @@ def kv_work_bytes(n_seq: int, n_pages: int) -> int:
 
 def kv_cache(k, v, table, length, ref, status, work) -> KvCache:
     """Describe a paged cache: pools k, v [page, head, key, dim] (any order of heads and keys in memory), table [sequence, page], length [sequence],
-    ref [page], status [1] int32, work: kv_work_bytes() bytes.  The arrays have to outlive the description."""
+    ref [page], status [1] int32, work: kv_work_bytes() bytes.  The description holds on to the arrays."""
     if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.dim() != 4 or str(k.dtype) not in _DTYPE or k.stride(3) != 1:
         raise ValueError("k and v: [page, head, key, dim] of one shape, type and layout, dims contiguous")
     if table.dim() != 2:
@@ -287,7 +287,7 @@ def kv_cache(k, v, table, length, ref, status, work) -> KvCache:
     c.nb_key, c.nb_head, c.nb_page = k.stride(2) * b, k.stride(1) * b, k.stride(0) * b
     c.table, c.len, c.ref = _ints(table, 0, "table"), _ints(length, c.n_seq, "length"), _ints(ref, c.n_pages, "ref")
     c.status, c.work = _ints(status, 1, "status"), work.data_ptr()
-    c.device = _device(k)
+    c.device, c.arrays = _device(k), (k, v, table, length, ref, status, work)
     return c
 
 
