@@ -8,8 +8,11 @@
 //                  S^T = K.Q^T and O^T = V^T.P^T on v_mfma_f32_32x32x16: a lane owns one row, so maximum, sum and rescaling are the lane's own scalars,
 //                  and P goes from registers to the second product.  K and V rows lie in LDS as they come, 16-byte pieces permuted so that neither the
 //                  row reads (K) nor the transposing reads (V) meet in a bank.  The two waves of a SIMD run half a step apart, one in the matrix products
-//                  (PV of the tile before, QK of this one) while the other is in the softmax: 8192 rows, 32 / 8 heads of 128, BF16: 546 us = 1007
-//                  TFLOP/s (585 on another card; both waves in step, and LDS rows at 8-byte addresses: 1555 us).
+//                  (PV of the tile before, QK of this one) while the other is in the softmax: 8192 rows, 32 / 8 heads of 128, BF16: 552 us = 997
+//                  TFLOP/s (531 to 588 by card; both waves in step, and LDS rows at 8-byte addresses: 1555 us).
+// Queries and weights are rounded to K's and V's type, which the matrix instructions take: half a step of 16 bits in each weight, whose sum is kept unrounded in 32, as
+// are maximum and result.  A second term of each weight would be the products with V once more, half as much matrix work again in a kernel that is bound by it.
+// What the rounding makes of infinities is put right by the writer (kinds_of).
 // A masked weight is an exact zero, but zero times an infinity or a NaN is none: where a tile that is masked in part holds such values, they are taken
 // out on the way into LDS and counted over the keys that a row sees, so that a row never meets what it does not see.
 #include "kv_cache.h"

@@ -16,7 +16,8 @@
 // range of keys.
 //
 // F32 queries are split into NT terms of the cache's type (2 x 11 or 3 x 8 bits), the weights likewise: the products are exact, the sums F32.  16-bit queries
-// take one term; the weights are then rounded to 16 bits, half a step of the result's own type.
+// take one term; the weights are then rounded to 16 bits, half a step of the result's own type (the sum of the weights is of the unrounded ones, in F32): an F16 or BF16
+// result is off by 2^-11 or 2^-8 either way.  Over a BF16 cache a step of F32 queries is thus finer than the same model's prompt (attn_packed.hip: one term).
 #include "kv_cache.h"
 
 #define TILE 32                        // keys of a tile: one 16x16x32 product over keys

@@ -267,9 +267,9 @@ __global__ void __launch_bounds__(KV_WG) k_kv_reserve(const KvAppendArgs a) {
 }
 
 // rows into their pages: rb rows per workgroup, whose places are looked up while the rows are on their way; behind them one workgroup per entry for shared
-// last pages.  Bound by HBM (rows in, rows out) once there are enough rows: with the two launches before it (9 us) 17321 rows of 8 heads of 128, 142 MB in
-// and out, 43.4 us, of which this is 27.5 (5.2 TB/s); four pieces of a thread at a time (eight: 46; places first, then the rows: 45, and 300 rows a sequence
-// 15.1 instead of 13.7; a bisection for each row: 32 rows 12.6, so 12.3).
+// last pages.  Bound by HBM (rows in, rows out) once there are enough rows: with the two launches before it (11 us) 17321 rows of 8 heads of 128, 142 MB in
+// and out, 43.1 us, of which this is about 32 (4.4 TB/s; 27.5 where the same rows come again and again); four pieces of a thread at a time (eight: 46; places first,
+// then the rows: 45, and 300 rows a sequence 15.1 instead of 13.7; a bisection for each row: 32 rows 12.6, so 12.4).
 #define KV_U 4
 #define KV_RB 16
 __global__ void __launch_bounds__(256) k_kv_write(const KvAppendArgs a) {

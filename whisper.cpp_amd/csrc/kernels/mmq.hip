@@ -20,7 +20,8 @@
 //    pair (first GPU run: 57 us for fc1, the f16 path 46) — is what bounds the kernel.  So (i) the integer sums arrive AS FLOATS: the
 //    MFMA's C operand is the constant 0x4B400000 in every element, i.e. D = bits(1.5 * 2^23) + sum, whose float value is 12582912 + sum
 //    exactly for |sum| < 2^22 (Q8_0 x Q8_0: 32 * 127 * 127 < 2^19), and 12582912 is subtracted again — exactly, float(sum) bit for bit —
-//    by a PACKED add; (ii) the fma is packed as well: 8 v_pk_add_f32 + 8 v_pk_fma_f32 = 64 cycles per MFMA pair.
+//    by one add; (ii) the fold is that add and one fma: 16 + 16 = 128 cycles per MFMA pair.  (In packed FP32, which this library is built without
+//    — build.py —, they would be 8 + 8 instructions.)
 //    The 32 x 32 tile of scale products dw[m]*dx[t] — 16 different
 //    weight rows per lane — comes from the matrix cores as well: one v_mfma_f32_32x32x16_f16 whose A operand holds dw (f16, exact) in
 //    K-slot 0 and whose B operand holds dx (an f16 value by construction of Q8_0) in K-slot 0, zeros elsewhere: a rank-1 product,
