@@ -328,6 +328,8 @@ class Ctx:
     def stream(self) -> int:
         """The stream (hipStream_t) that every call is launched on.  It waits for no other, torch's among them: work on the same arrays belongs on it too
         (torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream))), or events between the two."""
+        if not self.h:
+            raise RuntimeError("the context is closed")
         return lib().mi355x_ctx_stream(self.h)
 
     def check(self, rc: int, what: str = "op"):
