@@ -1235,3 +1235,109 @@ def test_prompts_and_a_compaction_captured_into_a_graph_and_replayed(gpu):
             assert torch.equal(x, y), rep
         for (_, pool, rest), (_, pool2, rest2) in zip(sets[0][1], sets[1][1]):
             assert all(torch.equal(x, y) for x, y in zip(pool + rest[:3], pool2 + rest2[:3])), rep
+
+
+@pytest.mark.parametrize("n", [64, 65, 4097, 20000])
+def test_thousands_of_sequences_in_one_call(gpu, n):
+    """of 0 to 3 rows: appended, attended to as packed rows (their own and the cache's, few and not) and one token each, where the searches have one, two and three levels"""
+    ctx, ka, torch = gpu
+    rng, gen, heads, dim, page = random.Random(n), torch.Generator(device="cuda").manual_seed(n), 2, 64, 4
+    counts = [rng.choice((0, 1, 2, 3)) for _ in range(n)]
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    total = int(cu[-1])
+    ints = lambda x: torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    zero = lambda *m: torch.zeros(*m, dtype=torch.int32, device="cuda")  # noqa: E731
+    q, k, v = (torch.randn(total, heads, dim, generator=gen, device="cuda").half() for _ in range(3))
+    pool = [torch.zeros(n, heads, page, dim, device="cuda").half() for _ in range(2)]
+    table, length, ref, status, work = zero(n, 2), zero(n), zero(n), zero(1), torch.empty(ka.kv_work_bytes(n, n), dtype=torch.uint8, device="cuda")
+    c = ka.kv_cache(*pool, table, length, ref, status, work)
+    # the definition: entry e's rows are cu[e] ..; row r of it sees the entry's rows up to itself, the one token all of them
+    starts = torch.tensor(cu[:-1], device="cuda")
+    entry = torch.repeat_interleave(torch.arange(n, device="cuda"), torch.tensor(counts, device="cuda"))
+    own = torch.arange(total, device="cuda") - starts[entry]
+
+    def define(rows, first, last):
+        """rows [R, heads, dim] over the keys first .. last (at most 3) of each; its allowed error as in expect(), with the larger of all bounds"""
+        at = (first[:, None] + torch.arange(3, device="cuda")).clamp_max(total - 1)
+        see = (torch.arange(3, device="cuda") <= (last - first)[:, None])[:, None]
+        x = (rows.double()[:, None] * k[at].double()).sum(3).transpose(1, 2) * 0.1
+        w = torch.softmax(torch.where(see, x, -math.inf), 2).nan_to_num(0.0)
+        o = (w[..., None] * v[at].double().transpose(1, 2)).sum(2)
+        e = 0.1 * float((rows.double().abs()[:, None] * k[at].double().abs()).sum(3).max()) * (dim + 8) * U["f32"]
+        return o, (math.expm1(4 * e) + 2 * U["f16"] + 40 * U["f32"]) * float(v.abs().max()) + U["f16"] * o.abs()
+
+    def hold(out, o, tol):
+        assert bool(((out.double() - o).abs() <= tol).all())
+
+    def run(call):
+        torch.cuda.synchronize()
+        call()
+        ctx.sync()
+
+    seq = rng.sample(range(n), n)
+    dseq, dcu = ints(seq), ints(cu)
+    run(ctx.kv_reset_call(c))
+    run(ctx.kv_append_call(c, dseq, dcu, k, v))
+    assert int(status) == 0
+    pages, t = iter(range(n)), table.tolist()
+    for e, s in enumerate(seq):
+        assert t[s] == ([next(pages), -1] if counts[e] else [-1, -1])
+    o, tol = define(q, starts[entry], starts[entry] + own)
+    for extra in (dict(k=k, v=v), dict(cache=c, seq=dseq)):
+        for max_q in (0, 3):
+            out = torch.full_like(q, 7.0)
+            run(ctx.attn_packed_call(q, out, dcu, scale=0.1, max_q=max_q, **extra))
+            hold(out, o, tol)
+    one = torch.randn(n, heads, dim, generator=gen, device="cuda").half()
+    out, space = torch.full_like(one, 7.0), torch.empty(max(16, ka.attn_paged_work_bytes(c, n, heads)), dtype=torch.uint8, device="cuda")
+    run(ctx.attn_paged_call(c, one, out, seq=dseq, scale=0.1, work=space))
+    o, tol = define(one, starts, starts + torch.tensor(counts, device="cuda") - 1)
+    hold(out, o, tol)
+
+
+@pytest.mark.parametrize("n", [4096, 4097])
+def test_one_long_sequence_among_thousands_of_short_ones(gpu, n):
+    """on both sides of the number of queries from which keys are not split"""
+    ctx, ka, torch = gpu
+    page, gen, long = 16, torch.Generator(device="cuda").manual_seed(n), 9001
+    lens = [i % 3 for i in range(n)]
+    lens[n // 2] = long
+    held = [-(-x // page) for x in lens]
+    k, v = (torch.randn(sum(held), 1, page, 64, generator=gen, device="cuda").half() for _ in range(2))
+    table, at = torch.full((n, max(held)), -1, dtype=torch.int32), 0
+    for s, h in enumerate(held):
+        table[s, :h] = torch.arange(at, at + h)
+        at += h
+    zero = lambda m: torch.zeros(m, dtype=torch.int32, device="cuda")  # noqa: E731
+    status = zero(1)
+    c = ka.kv_cache(k, v, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), zero(sum(held)), status, torch.empty(ka.kv_work_bytes(n, sum(held)), dtype=torch.uint8, device="cuda"))
+    q = torch.randn(n, 3, 64, generator=gen, device="cuda").half()
+    out, need = torch.full_like(q, 7.0), ka.attn_paged_work_bytes(c, n, 3)
+    assert (need > 0) == (n <= 4096)
+    space = torch.empty(max(16, need), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    ctx.attn_paged_call(c, q, out, scale=0.125, work=space)()
+    ctx.sync()
+    assert int(status) == 0
+    for s in [0, 1, 2, 3, n // 2 - 1, n // 2, n // 2 + 1, n - 3, n - 2, n - 1]:
+        flat = [x.cpu()[table[s, : held[s]].long()].transpose(1, 2).reshape(-1, 1, 64)[: lens[s]] for x in (k, v)]
+        o, tol = expect(torch, q[s].cpu(), *flat, torch.ones(lens[s], dtype=torch.bool), 0.125, "f16", "f16", "f16", False, True)
+        same(torch, out[s], o, tol)
+
+
+@pytest.mark.parametrize("kind,io", [("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("dim,rows,max_q", [(64, 9, 8), (128, 9, 0), (64, 300, 0), (128, 300, 0)])
+def test_queries_and_results_inside_larger_arrays(gpu, kind, io, dim, rows, max_q):
+    """every third head of a projection's rows, every second row of a result: what lies between is as it was"""
+    ctx, ka, torch = gpu
+    p = Pool(gpu, n_seq=rows, n_pages=40, max_pages=30, page=16, heads=2, dim=dim, kind=kind)
+    assert p.append([(1, 400), (2, 30)], kind) == 0
+    wide = torch.randn(2 * rows, 20, dim, generator=p.gen, device="cuda").to(dt(torch, io))
+    q = wide[::2, 1:17:3]                                            # 6 heads
+    seq = p.ints([1, 2, -1] * (rows // 3))
+    for call in (lambda q, o: ctx.attn_paged_call(p.c, q, o, seq=seq, scale=0.1), lambda q, o: ctx.attn_packed_call(q, o, p.ints([0, rows]), cache=p.c, seq=p.ints([1]), scale=0.1, max_q=max_q)):
+        plain, big = torch.zeros(rows, 6, dim, device="cuda"), torch.full((2 * rows, 13, dim), 7.0, device="cuda")
+        p.run(call(q.contiguous(), plain))
+        p.run(call(q, big[1::2, 1::2]))
+        assert torch.equal(big[1::2, 1::2], plain) and float(plain.abs().max()) > 0
+        assert (big[::2] == 7).all() and (big[:, ::2] == 7).all()
